@@ -17,6 +17,7 @@ from . import ops
 
 GROUPS = (32, 64, 128)
 TYPES = (torch.float32, torch.bfloat16)
+MAX_COLUMNS = 32768
 
 _quantize = _linear = None
 
@@ -25,8 +26,8 @@ def _bind():
     global _quantize, _linear
     if _linear is None:
         _quantize = ops.bind("qs_q4_quantize", [c_void_p, c_void_p, c_void_p, c_int, c_longlong, c_int, c_int, c_int, c_void_p])
-        _linear = ops.bind("qs_q4_linear", [c_void_p, c_int, c_longlong, c_void_p, c_int, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_int,
-                                            c_void_p, c_void_p, c_longlong, c_int, c_int, c_int, c_int, c_void_p])
+        _linear = ops.bind("qs_q4_linear", [c_void_p, c_int, c_longlong, c_void_p, c_int, c_longlong, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                                            c_void_p, c_void_p, c_longlong, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p])
 
 
 def _refuse(text, code=QsError.INVALID_INPUT):
@@ -109,10 +110,11 @@ def quantize(weight: torch.Tensor, group: int = 64) -> Weight4:
     return Weight4(codes, scales, N, K, group)
 
 
-def linear(x, weight: Weight4, bias=None, activation=None, residuals=(), out_dtype=None, out=None) -> torch.Tensor:
+def linear(x, weight: Weight4, bias=None, activation=None, residuals=(), out_dtype=None, out=None, settled=False) -> torch.Tensor:
     """act(x W^T + bias) + residuals for rows x [M, in_features] of float32 or bfloat16, accumulated in 32 bits.  Arguments and
     result as for `parts.linear.linear`: up to two residuals of x's type; `out_dtype` float32 for a 32-bit result; `out`: a view to
-    write into (contiguous rows, any row stride)."""
+    write into (contiguous rows, any row stride).  `settled`: the weight was complete before the previous kernel of the stream began
+    (a model's is); the kernel then fetches it while that kernel still runs."""
     M, K, ldx = ops._rows(x)
     N = weight.out_features
     if K != weight.in_features:
@@ -126,12 +128,20 @@ def linear(x, weight: Weight4, bias=None, activation=None, residuals=(), out_dty
     want = out.dtype if out is not None else out_dtype or x.dtype
     if want not in ((torch.float32,) if x.dtype == torch.float32 else TYPES) or (out is not None and out_dtype not in (None, out.dtype)):
         _refuse(f"linear: a result of {want} from rows of {x.dtype}")
+    if K > MAX_COLUMNS:
+        _refuse(f"linear: {K} columns, the kernels take {MAX_COLUMNS}")
     out, res, ldr = ops._product_views(x, M, N, [r for r in residuals if r is not None], want, out)
     if M == 0:
         return out
     _on_current_device(x, weight.codes, bias, out, *res[:2])
     _bind()
-    ops.check(_linear(ops.ptr(out), ops.dtype_code(out), out.stride(0), ops.ptr(x), ops.dtype_code(x), ldx, ops.ptr(weight.codes), ops.ptr(weight.scales),
+    code, element = ops.dtype_code(x), x.element_size()
+    aligned = x.data_ptr() % 16 == 0 and ldx * element % 16 == 0
+    scratch = None
+    if code == ops.F32 or K % 64 or not aligned:        # rows laid out anew: whole chunks of 64 columns, three terms to a float32 number
+        scratch = torch.empty((M * (3 if code == ops.F32 else 1), -(-K // 64) * 64), dtype=torch.bfloat16, device=x.device)
+        ops.count_launches(1)
+    ops.check(_linear(ops.ptr(out), ops.dtype_code(out), out.stride(0), ops.ptr(x), code, ldx, int(aligned), ops.ptr(weight.codes), ops.ptr(weight.scales),
                       ops.ptr(bias), ops.dtype_code(bias) if bias is not None else 0, ops.ACTIVATIONS[activation], ops.ptr(res[0]), ops.ptr(res[1]), ldr,
-                      M, N, K, weight.group, ops.stream()))
+                      M, N, K, weight.group, int(bool(settled)), ops.ptr(scratch), ops.stream()))
     return out

@@ -152,3 +152,22 @@ def test_on_another_stream_and_in_a_graph():
                 g.replay()
     torch.cuda.synchronize()
     assert torch.equal(outs[0], want) and torch.equal(outs[1], -want)
+
+
+def test_a_float32_row_is_the_same_bits_in_any_batch():
+    for k, group in ((2048, 64), (700, 32), (5000, 128)):
+        w = q4.quantize(normal(k, 90, k, std=0.1), group)
+        x = normal(2, 70, k)
+        whole = q4.linear(x, w)
+        for m in (1, 2, 3, 5, 6, 16, 33):
+            assert torch.equal(q4.linear(x[:m], w), whole[:m])
+
+
+@pytest.mark.parametrize("n,k", [(70, 16500), (33, 32768), (20, 9000)])
+def test_many_columns(n, k):
+    w = q4.quantize(normal(1, n, k, std=0.02), 64)
+    for dtype in TYPES.values():
+        for m in (1, 5, 12, 40):
+            x = normal(m, m, k, dtype=dtype)
+            want, bound = U.linear(U.f64(x), U.dense(w), out_bf16=dtype == torch.bfloat16)
+            assert (np.abs(U.f64(q4.linear(x, w)) - want) <= bound).all(), m

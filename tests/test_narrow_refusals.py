@@ -45,6 +45,8 @@ def test_products_that_are_refused():
                dict(out=torch.zeros(3, 40).bfloat16()), dict(out=torch.zeros(40, 3).t()), dict(out=ok, out_dtype=torch.bfloat16), dict(x=x)):
         refused(QsError.INVALID_INPUT, q4.linear, **{**dict(x=x, weight=w), **kw})
     assert q4.linear(x[:0], w).shape == (0, 40)
+    wide = weight(16, 40000, 128)
+    refused(QsError.INVALID_INPUT, q4.linear, torch.zeros(1, 40000), wide)
 
 
 I = lambda *s: torch.zeros(s, dtype=torch.int32)           # noqa: E731,E741
