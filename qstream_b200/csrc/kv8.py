@@ -16,17 +16,22 @@ from . import ops
 from .q4 import TYPES, _on_current_device, _refuse
 
 PAGE_TOKENS = 64
+MAX_SPLIT_CONTEXT = 4096 * 128      # what the merge of the keys' parts holds for any head size; longer contexts go a row at a time
 
-_store = _read = _attention = None
+_store = _read = _attention = _decode = _splits = None
 
 
 def _bind():
-    global _store, _read, _attention
+    global _store, _read, _attention, _decode, _splits
     if _store is None:
         _read = ops.bind("qs_kv8_read_pages", [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p])
         _attention = ops.bind("qs_kv8_attention", [
             c_void_p, c_int, c_longlong, c_void_p, c_int, c_longlong, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int,
             c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p, c_float, c_int, c_void_p, c_void_p])
+        _decode = ops.bind("qs_kv8_decode", [
+            c_void_p, c_int, c_longlong, c_void_p, c_int, c_longlong, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+            c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p, c_float, c_int, c_void_p, c_void_p, c_void_p])
+        _splits = ops.bind("qs_kv8_decode_splits", [c_int, c_int, c_int])
         _store = ops.bind("qs_kv8_store", [
             c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong, c_float, c_int,
             c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
@@ -166,6 +171,16 @@ def decode(q, n_heads, n_kv_heads, head_dim, scale, window, tok_slot, tok_pos, p
     _on_current_device(q, out, tok_slot, tok_pos, page_table, k_cache, v_cache, k_scale, v_scale, status, sink)
     ops.ptr(q)
     _bind()
+    if head_dim % 16 == 0 and dv % 16 == 0 and head_dim <= 256 and dv <= 256 and T <= 65535 and max_context <= MAX_SPLIT_CONTEXT:
+        splits = _splits(head_dim, dv, max_context)
+        partial = torch.empty((T * n_heads * splits * (dv + 2),), dtype=torch.float32, device=q.device) if splits > 1 else None
+        ops.check(_decode(ops.ptr(out), int(out.dtype == torch.float32), out.stride(0), ops.ptr(q), ops.dtype_code(q), q.stride(0), T, ops.ptr(tok_slot), ops.ptr(tok_pos),
+                          ops.ptr(page_table), page_table.shape[0], page_table.shape[1], k_cache.shape[0], ops.ptr(k_cache), ops.ptr(v_cache), ops.ptr(k_scale),
+                          ops.ptr(v_scale), n_heads, n_kv_heads, head_dim, dv, float(scale), int(window), int(chunk), int(keep_first), ops.ptr(sink),
+                          float(softcap or 0.0), int(max_context), ops.ptr(partial), ops.ptr(status), ops.stream()))
+        if partial is not None:
+            ops.count_launches(1)                       # split kernel + merge kernel
+        return out
     for a in range(0, T, 65535):
         b = min(T, a + 65535)
         ops.check(_attention(ops.ptr(out[a:b]), ops.dtype_code(out), out.stride(0), ops.ptr(q[a:b]), ops.dtype_code(q), q.stride(0), b - a, ops.ptr(tok_slot[a:b]),
