@@ -2,14 +2,14 @@
 //
 //   s[u] = scale * q.K[u] (capped), K[u] = code * scale of u's page;  softmax over the keys that the mask leaves;  o = sum_u p[u] V[u]
 //
-// Bound by the bytes of the pages.  A warp takes one page of 64 keys and up to HEADS query heads that share its key head: two bulk
-// copies bring the page's keys and values into shared memory (all pages of a block are on their way at once, from the first instruction
-// on), 16-bit products on mma.m16n8k16 take them from there.
+// Bound by the bytes of the pages.  A warp takes 32 keys (16 of wide heads) and up to HEADS query heads that share their key head: two
+// bulk copies bring keys and values into shared memory (all of a block are on their way at once, from the first instructions on),
+// 16-bit products on mma.m16n8k16 take them from there.
 //
 //   scores   left operand: 16 keys, right: the heads.  A lane's 16 bytes of a key's row are its part of four steps; which dims meet in
 //            a step is free, so the queries are laid out the same way.  A code, as the low byte of a 16-bit float 1024 beside its upper
 //            byte, is 1024 + 128 + code once its sign bit is flipped, and 1152 less the code, exactly.  The page's scale joins the 32-bit score.
-//   weights  p = 2^(s - m + 15), m the page's own maximum: 16-bit floats from 2^15 down to 2^-24 hold weights of 2^-29 and more with all
+//   weights  p = 2^(s - m + 15), m the warp's own maximum: 16-bit floats from 2^15 down to 2^-24 hold weights of 2^-29 and more with all
 //            11 bits, and the rest to 2^-40.
 //   values   left operand: 16 dims of the values' transpose, right: the heads' weights, turned by movmatrix from the scores' layout.  Row g of
 //            tile j is dim 16 g + 2 j, row g + 8 the next: a lane's 16 bytes of a key are its part of eight tiles.  The page's scale joins the sums.
@@ -28,18 +28,20 @@
 
 namespace {
 
-constexpr int PAGE = 64;
+constexpr int PAGE = 64, WARPS = 8;
 
 struct DecodeArgs {
     void* out;
-    float* partial;                                      // [rows][heads][splits][dv + 2]
+    float* partial;                                      // [rows][heads][splits][dv]
+    float2* ml;                                          // [rows][heads][splits]: maximum (base two), sum
     const void* q;
     const int8_t *k_cache, *v_cache;
     const float *k_scale, *v_scale, *sink;
     const int32_t *tok_slot, *tok_pos, *page_table;
     size_t ldo, ldq;
     int max_pages, n_slots, n_pages, n_heads, n_kv_heads, dk, dv, window, chunk, keep_first, splits, out_f32;
-    float scale, softcap;
+    float scale, softcap, cap_k2;
+    int q_aligned;
     int32_t* status;
 };
 
@@ -89,15 +91,16 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                  ::"r"(sm100::smem_u32(dst)), "l"(src), "r"(bytes), "r"(sm100::smem_u32(bar)) : "memory");
 }
 
-// KC: blocks of 64 dims that keys span at most; VB: blocks of 128 dims of the values; WARPS pages to a block.
-template <typename T, int KC, int VB, int WARPS>
+// KC: blocks of 64 dims that keys span at most; VB: blocks of 128 dims of the values; a warp takes KEYS keys.
+template <typename T, int KC, int VB, int KEYS>
 __global__ void __launch_bounds__(WARPS * 32)
 kv8_decode_kernel(const DecodeArgs p) {
     constexpr bool WIDE = sizeof(T) == 4;                // two columns to a head
-    constexpr int HEADS = WIDE ? 4 : 8, SPLIT = WARPS * PAGE;
-    extern __shared__ __align__(128) uint8_t smem[];     // per warp: its page's keys, its values; in the end [WARPS][HEADS][dv] sums
+    constexpr int HEADS = WIDE ? 4 : 8, SPLIT = WARPS * KEYS, TILES = KEYS / 16;
+    extern __shared__ __align__(128) uint8_t smem[];     // per warp: its keys, its values; in the end [WARPS][HEADS][dv] sums
     __shared__ uint64_t bars[WARPS][2];
-    __shared__ float s_m[WARPS][HEADS], s_l[WARPS][HEADS];
+    __shared__ float s_m[WARPS][HEADS], s_l[WARPS][HEADS], s_unit[8];
+    __shared__ uint32_t s_q[KC * 8][32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     grid_dep_launch();
     if (lane == 0) {
@@ -121,72 +124,59 @@ kv8_decode_kernel(const DecodeArgs p) {
     const int first = first_key(p, pos), keep = p.window > 0 ? min(p.keep_first, first) : 0;
     const int base = split * SPLIT;
     if (base > pos || (base + SPLIT <= first && base >= keep)) return;       // no key of this split is seen
-    const int key0 = base + warp * PAGE;
-    const bool seen = key0 <= pos && (key0 + PAGE > first || key0 < keep);
+    const int key0 = base + warp * KEYS;
+    const bool seen = key0 <= pos && (key0 + KEYS > first || key0 < keep);
     int page = -1;
     if (seen) {
         page = p.page_table[(size_t)slot * p.max_pages + (key0 >> 6)];
         if (page < 0 || page >= p.n_pages) { if (lane == 0) atomicExch(p.status, 3); page = -1; }
     }
-    const int page_bytes = PAGE * (p.dk + p.dv) + 128;   // rows are read in whole blocks of dims: up to 127 bytes beyond the last
-    uint8_t* keys = smem + warp * page_bytes;
-    uint8_t* values = keys + PAGE * p.dk;
+    const int warp_bytes = KEYS * (p.dk + p.dv) + 128;   // rows are read in whole blocks of dims: up to 127 bytes beyond the last
+    uint8_t* keys = smem + warp * warp_bytes;
+    uint8_t* values = keys + KEYS * p.dk;
     const size_t at = (size_t)max(page, 0) * p.n_kv_heads + kvh;
     if (page >= 0 && lane == 0) {
-        const int n = min(PAGE, pos - key0 + 1);         // rows behind the sequence's end stay out of it
+        const int n = min(KEYS, pos - key0 + 1);         // rows behind the sequence's end stay out of it
+        const size_t in_page = at * PAGE + (key0 & (PAGE - 1));
         sm100::mbar_expect_tx(&bars[warp][0], n * p.dk);
-        bulk_load(keys, p.k_cache + at * PAGE * p.dk, n * p.dk, &bars[warp][0]);
+        bulk_load(keys, p.k_cache + in_page * p.dk, n * p.dk, &bars[warp][0]);
         sm100::mbar_expect_tx(&bars[warp][1], n * p.dv);
-        bulk_load(values, p.v_cache + at * PAGE * p.dv, n * p.dv, &bars[warp][1]);
+        bulk_load(values, p.v_cache + in_page * p.dv, n * p.dv, &bars[warp][1]);
     }
     const float ks = page >= 0 ? p.k_scale[at] : 0.f, vs = page >= 0 ? p.v_scale[at] : 0.f;
 
-    // the queries: column g is head g (WIDE: head g & 3, its first or second term), dims 64 c + 16 t .. + 15
-    uint32_t qf[KC][8];
-    float q_unit = 0.f;                                  // what one of column g's numbers stands for
+    // The queries, laid out for all warps: warp w makes column w, which is head w (WIDE: head w & 3, its first or second term); lane l
+    // its dims 8 l .. 8 l + 7.  A lane of the products has dims 64 c + 16 t .. + 15 of column g.
     {
-        const int h = WIDE ? g & 3 : g;
-        const T* src = reinterpret_cast<const T*>(p.q) + (size_t)row * p.ldq + (size_t)(head0 + min(h, heads - 1)) * p.dk;
+        const T* src = reinterpret_cast<const T*>(p.q) + (size_t)row * p.ldq + (size_t)(head0 + min(WIDE ? warp & 3 : warp, heads - 1)) * p.dk + 8 * lane;
+        float x[8];
+        if (8 * lane < p.dk && p.q_aligned) load8_as_f32(src, WIDE ? QS_F32 : QS_BF16, 0, x);
+        else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = 8 * lane + i < p.dk ? to_f32(src[i]) : 0.f;
+        }
         float most = 0.f;
-        float f[WIDE ? 1 : KC][WIDE ? 1 : 16];
 #pragma unroll
-        for (int c = 0; c < KC; ++c)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int d = 64 * c + 16 * t + i;
-                const float x = d < p.dk ? to_f32(src[d]) : 0.f;
-                if (!WIDE) f[WIDE ? 0 : c][WIDE ? 0 : i] = x;
-                most = fmaxf(most, fabsf(x));
-            }
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[i]));
+        most = warp_max(most);
         // the power of two at or below the largest; numbers that are not finite go through as they are
         const uint32_t e = min(max(__float_as_uint(most) >> 23, 1u), 253u);
-        q_unit = __uint_as_float(e << 23);
         const float inv = __uint_as_float((254u - e) << 23);
+        if (lane == 0) s_unit[warp] = __uint_as_float(e << 23);
 #pragma unroll
-        for (int c = 0; c < KC; ++c)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float x[2];
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int d = 64 * c + 16 * t + 2 * i + j;
-                    x[j] = (WIDE ? (d < p.dk ? to_f32(src[d]) : 0.f) : f[WIDE ? 0 : c][WIDE ? 0 : 2 * i + j]) * inv;
-                }
-                uint32_t v = pack_f16(x[0], x[1]);
-                if (WIDE && g >= 4) {
-                    const float2 hi = unpack_f16(v);
-                    v = pack_f16(x[0] - hi.x, x[1] - hi.y);
-                }
-                qf[c][i] = v;
+        for (int i = 0; i < 4; ++i) {
+            uint32_t v = pack_f16(x[2 * i] * inv, x[2 * i + 1] * inv);
+            if (WIDE && warp >= 4) {
+                const float2 hi = unpack_f16(v);
+                v = pack_f16(x[2 * i] * inv - hi.x, x[2 * i + 1] * inv - hi.y);
             }
+            if (lane < KC * 8) s_q[(lane >> 3) * 8 + (lane & 1) * 4 + i][warp * 4 + (lane >> 1 & 3)] = v;
+        }
     }
+    __syncthreads();
     // of the columns that this lane's results belong to: 2 t, 2 t + 1 (WIDE: of their heads, in both halves)
     const int h0 = WIDE ? 2 * (t & 1) : 2 * t;
-    float unit[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) unit[j] = __shfl_sync(0xffffffffu, q_unit, (h0 + j) * 4) * ks * p.scale;
+    const float unit[2] = {s_unit[h0] * ks * p.scale, s_unit[h0 + 1] * ks * p.scale};
 
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
     float acc[VB * 8][4];
@@ -195,43 +185,57 @@ kv8_decode_kernel(const DecodeArgs p) {
     const bool ok = page >= 0 && sm100::mbar_wait(&bars[warp][0], 0);
     if (page >= 0 && !ok && lane == 0) atomicExch(p.status, 123);
     if (ok) {
-        // scores of the page's 64 keys: tile i, row g (and g + 8) is key 16 i + g (+ 8)
-        float s[4][4];
+        // scores of the keys: tile i, row g (and g + 8) is key 16 i + g (+ 8)
+        float s[TILES][4];
         const float log2e = 1.4426950408889634f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+        for (int i = 0; i < TILES; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
 #pragma unroll
-            for (int c = 0; c < KC; ++c) {
-                if (64 * c >= p.dk) break;
+        for (int c = 0; c < KC; ++c) {
+            if (64 * c >= p.dk) break;
+            uint32_t qf[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) qf[i] = s_q[c * 8 + i][lane];
+#pragma unroll
+            for (int i = 0; i < TILES; ++i) {
                 const uint4 lo = *reinterpret_cast<const uint4*>(keys + (16 * i + g) * p.dk + 64 * c + 16 * t);
                 const uint4 hi = *reinterpret_cast<const uint4*>(keys + (16 * i + g + 8) * p.dk + 64 * c + 16 * t);
                 const uint32_t a[4] = {lo.x ^ 0x80808080u, lo.y ^ 0x80808080u, lo.z ^ 0x80808080u, lo.w ^ 0x80808080u};
                 const uint32_t b[4] = {hi.x ^ 0x80808080u, hi.y ^ 0x80808080u, hi.z ^ 0x80808080u, hi.w ^ 0x80808080u};
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    mma_sum<WIDE>(s[i], two_codes(a[k], 0x4140), two_codes(b[k], 0x4140), two_codes(a[k], 0x4342), two_codes(b[k], 0x4342), qf[c][2 * k], qf[c][2 * k + 1]);
+                    mma_sum<WIDE>(s[i], two_codes(a[k], 0x4140), two_codes(b[k], 0x4140), two_codes(a[k], 0x4342), two_codes(b[k], 0x4342), qf[2 * k], qf[2 * k + 1]);
             }
+        }
+        const bool whole = key0 + KEYS - 1 <= pos && (key0 >= first || key0 + KEYS <= keep);
+#pragma unroll
+        for (int i = 0; i < TILES; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int key = key0 + 16 * i + g + 8 * (e >> 1);
                 float x = s[i][e];
                 if (WIDE) x += __shfl_xor_sync(0xffffffffu, x, 2);
                 x *= unit[e & 1];
-                if (p.softcap > 0.f) x = p.softcap * tanhf(x / p.softcap);
-                s[i][e] = key <= pos && (key >= first || key < keep) ? x * log2e : -INFINITY;
-                m[e & 1] = fmaxf(m[e & 1], s[i][e]);
+                if (p.softcap > 0.f) {
+                    if (WIDE) x = p.softcap * tanhf(x / p.softcap);
+                    else x = p.softcap - __fdividef(2.f * p.softcap, fast_exp2(x * p.cap_k2) + 1.f);      // tanh u = 1 - 2 / (e^2u + 1), within 10^-6 of the cap
+                }
+                x *= log2e;
+                if (!whole) {
+                    const int key = key0 + 16 * i + g + 8 * (e >> 1);
+                    if (key > pos || (key < first && key >= keep)) x = -INFINITY;
+                }
+                s[i][e] = x;
+                m[e & 1] = fmaxf(m[e & 1], x);
             }
-        }
         // the weights, in pairs of heads; the columns' maxima and sums over the eight lanes of a column
-        uint32_t w[4][2];                                // tile i, rows g and g + 8: two heads
+        uint32_t w[TILES][2];                            // tile i, rows g and g + 8: two heads
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) m[j] = fmaxf(m[j], __shfl_xor_sync(0xffffffffu, m[j], o));
         const float zero[2] = {m[0] == -INFINITY ? 0.f : m[0] - 15.f, m[1] == -INFINITY ? 0.f : m[1] - 15.f};     // all -inf (or NaN): 2^-inf is 0
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < TILES; ++i)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 float a = fast_exp2(s[i][2 * e] - zero[0]), b = fast_exp2(s[i][2 * e + 1] - zero[1]);
@@ -250,7 +254,7 @@ kv8_decode_kernel(const DecodeArgs p) {
             for (int o = 4; o < 32; o <<= 1) l[j] += __shfl_xor_sync(0xffffffffu, l[j], o);
         if (sm100::mbar_wait(&bars[warp][1], 0)) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)                  // 16 keys: this lane's are 2 t, 2 t + 1 and the same + 8
+            for (int i = 0; i < TILES; ++i)              // 16 keys: this lane's are 2 t, 2 t + 1 and the same + 8
 #pragma unroll
                 for (int b = 0; b < VB; ++b) {
                     if (128 * b >= p.dv) break;
@@ -276,113 +280,157 @@ kv8_decode_kernel(const DecodeArgs p) {
     }
     // The warps' results: sums as [head][dim], beside each other where the pages were.
     if (g == 0 && (!WIDE || t < 2)) { s_m[warp][h0] = m[0]; s_m[warp][h0 + 1] = m[1]; s_l[warp][h0] = l[0]; s_l[warp][h0 + 1] = l[1]; }
-    __syncthreads();                                     // everybody has read its page
+    __syncthreads();                                     // everybody has read its keys and values
     float* sums = reinterpret_cast<float*>(smem);
+    // what a warp's sums count beside the others'; a warp without a key that is seen: nothing; one whose scores are all NaN: NaN
+    float M[2] = {-INFINITY, -INFINITY}, a[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) M[j] = fmaxf(M[j], s_m[w][h0 + j]);
+        a[j] = (m[j] == -INFINITY ? 1.f : exp2f(m[j] - M[j]));
+    }
 #pragma unroll
     for (int j = 0; j < VB * 8; ++j) {
         const int d = (j >> 3) * 128 + 16 * g + 2 * (j & 7);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             if (WIDE) acc[j][e] += __shfl_xor_sync(0xffffffffu, acc[j][e], 2);
-            acc[j][e] = page >= 0 ? acc[j][e] * vs : 0.f;
+            acc[j][e] = page >= 0 ? acc[j][e] * vs * a[e & 1] : 0.f;
         }
         if (d < p.dv && (!WIDE || t < 2)) {
-            *reinterpret_cast<float2*>(sums + (warp * HEADS + h0) * p.dv + d) = make_float2(acc[j][0], acc[j][2]);
-            *reinterpret_cast<float2*>(sums + (warp * HEADS + h0 + 1) * p.dv + d) = make_float2(acc[j][1], acc[j][3]);
+            if (h0 < heads) *reinterpret_cast<float2*>(sums + (warp * HEADS + h0) * p.dv + d) = make_float2(acc[j][0], acc[j][2]);
+            if (h0 + 1 < heads) *reinterpret_cast<float2*>(sums + (warp * HEADS + h0 + 1) * p.dv + d) = make_float2(acc[j][1], acc[j][3]);
         }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < heads * p.dv; i += WARPS * 32) {
-        const int h = i / p.dv, d = i - h * p.dv;
-        float M = -INFINITY, L = 0.f, o = 0.f;
+    if (warp < heads) {                                  // a head to a warp
+        for (int h = warp; h < heads; h += WARPS) {
+            float Mh = -INFINITY, L = 0.f;
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) M = fmaxf(M, s_m[w][h]);
+            for (int w = 0; w < WARPS; ++w) Mh = fmaxf(Mh, s_m[w][h]);
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) {                // a page without a key that is seen: nothing; one whose scores are all NaN: NaN
-            const float a = s_m[w][h] == -INFINITY ? 1.f : exp2f(s_m[w][h] - M);
-            L += s_l[w][h] * a;
-            o += sums[(w * HEADS + h) * p.dv + d] * a;
-        }
-        if (p.splits == 1) {
-            // as the merge of one split
-            if (p.sink) {
-                const float sink = p.sink[head0 + h] * 1.4426950408889634f, all = fmaxf(M, sink), a = M == -INFINITY ? 1.f : exp2f(M - all);
-                L = fmaf(L, a, exp2f(sink - all + 15.f));
-                o *= a;
+            for (int w = 0; w < WARPS; ++w) L = fmaf(s_l[w][h], s_m[w][h] == -INFINITY ? 1.f : exp2f(s_m[w][h] - Mh), L);
+            float factor = 1.f;
+            if (p.splits == 1) {                         // as the merge of one split
+                if (p.sink) {
+                    const float sink = p.sink[head0 + h] * 1.4426950408889634f, all = fmaxf(Mh, sink);
+                    factor = Mh == -INFINITY ? 1.f : exp2f(Mh - all);
+                    L = fmaf(L, factor, exp2f(sink - all + 15.f));
+                }
+                factor *= L != 0.f ? 1.0f / L : 0.f;
             }
-            store_from_f32(p.out, p.out_f32 ? QS_F32 : QS_BF16, (size_t)row * p.ldo + (size_t)(head0 + h) * p.dv + d, o * (L != 0.f ? 1.0f / L : 0.f));
-        } else {
-            float* to = p.partial + (((size_t)row * p.n_heads + head0 + h) * p.splits + split) * (p.dv + 2);
-            to[d] = o;
-            if (d == 0) { to[p.dv] = M; to[p.dv + 1] = L; }
+            const size_t cell = ((size_t)row * p.n_heads + head0 + h) * p.splits + split;
+            for (int d = 4 * lane; d < p.dv; d += 128) {
+                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < WARPS; ++w) {
+                    const float4 v = *reinterpret_cast<const float4*>(sums + (w * HEADS + h) * p.dv + d);
+                    o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
+                }
+                if (p.splits > 1) {
+                    *reinterpret_cast<float4*>(p.partial + cell * p.dv + d) = o;
+                } else {
+                    const size_t to = (size_t)row * p.ldo + (size_t)(head0 + h) * p.dv + d;
+                    const int type = p.out_f32 ? QS_F32 : QS_BF16;
+                    store_from_f32(p.out, type, to, o.x * factor);
+                    store_from_f32(p.out, type, to + 1, o.y * factor);
+                    store_from_f32(p.out, type, to + 2, o.z * factor);
+                    store_from_f32(p.out, type, to + 3, o.w * factor);
+                }
+            }
+            if (p.splits > 1 && lane == 0) p.ml[cell] = make_float2(Mh, L);
         }
     }
 }
 
-// One block per row and head: the splits' results in ascending order.
+// One block per row and head: the splits' results.  The threads of a group have four dims each; the groups share the splits, each in
+// ascending order, and are added in theirs; how the splits are shared depends on their number for the row and on dv.
+constexpr int MERGE_THREADS = 256;
 template <int SPLIT>
-__global__ void kv8_merge_kernel(const DecodeArgs p) {
-    extern __shared__ float s_all[];                     // [splits] weights, [splits] sums
+__global__ void __launch_bounds__(MERGE_THREADS)
+kv8_merge_kernel(const DecodeArgs p) {
+    extern __shared__ float s_w[];                       // [splits] weights
+    __shared__ float scratch[34];
+    __shared__ __align__(16) float4 s_o[MERGE_THREADS];
     grid_dep_launch();
     grid_dep_wait();
-    const int head = blockIdx.x, row = blockIdx.y, dv = p.dv;
-    const int slot = p.tok_slot[row], pos = p.tok_pos[row];
+    const int head = blockIdx.x, row = blockIdx.y, dv = p.dv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int slot = p.tok_slot[row], pos = p.tok_pos[row], type = p.out_f32 ? QS_F32 : QS_BF16;
     const size_t to = (size_t)row * p.ldo + (size_t)head * dv;
     if (slot < 0 || slot >= p.n_slots || pos < 0 || (pos >> 6) >= p.max_pages || pos >= p.splits * SPLIT) {       // padding, or reported: a defined row
-        for (int d = threadIdx.x; d < dv; d += blockDim.x) store_from_f32(p.out, p.out_f32 ? QS_F32 : QS_BF16, to + d, 0.f);
+        for (int d = threadIdx.x; d < dv; d += MERGE_THREADS) store_from_f32(p.out, type, to + d, 0.f);
         return;
     }
     const int first = first_key(p, pos), keep = p.window > 0 ? min(p.keep_first, first) : 0;
     // the splits with keys that are seen: those of the kept first keys, then those of the window
     const int kept = keep > 0 ? (keep - 1) / SPLIT + 1 : 0, lo = max(first / SPLIT, kept), n = kept + pos / SPLIT - lo + 1;
-    const float* base = p.partial + ((size_t)row * p.n_heads + head) * p.splits * (dv + 2);
-    auto part = [&](int i) { return base + (size_t)(i < kept ? i : lo + i - kept) * (dv + 2); };
-    __shared__ float scratch[33];
-    float M = p.sink ? p.sink[head] * 1.4426950408889634f : -INFINITY;
-    for (int i = threadIdx.x; i < n; i += blockDim.x) {
-        s_all[i] = part(i)[dv];
-        s_all[n + i] = part(i)[dv + 1];
-        M = fmaxf(M, s_all[i]);
+    const size_t cell = ((size_t)row * p.n_heads + head) * p.splits;
+    auto split = [&](int i) { return i < kept ? i : lo + i - kept; };
+    float M = p.sink ? p.sink[head] * 1.4426950408889634f : -INFINITY, L = 0.f;
+    for (int i = threadIdx.x; i < n; i += MERGE_THREADS) {
+        const float m = p.ml[cell + split(i)].x;
+        s_w[i] = m;
+        M = fmaxf(M, m);
     }
     M = warp_max(M);
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = M;
+    if (lane == 0) scratch[warp] = M;
     __syncthreads();
-    for (int i = 0; i < (int)(blockDim.x >> 5); ++i) M = fmaxf(M, scratch[i]);
-    for (int i = threadIdx.x; i < n; i += blockDim.x) s_all[i] = s_all[i] == -INFINITY ? 1.f : exp2f(s_all[i] - M);
+#pragma unroll
+    for (int i = 0; i < MERGE_THREADS / 32; ++i) M = fmaxf(M, scratch[i]);
     __syncthreads();
-    float L = p.sink ? exp2f(p.sink[head] * 1.4426950408889634f - M + 15.f) : 0.f;
-    for (int i = 0; i < n; ++i) L = fmaf(s_all[n + i], s_all[i], L);
+    for (int i = threadIdx.x; i < n; i += MERGE_THREADS) {
+        s_w[i] = s_w[i] == -INFINITY ? 1.f : exp2f(s_w[i] - M);
+        L = fmaf(p.ml[cell + split(i)].y, s_w[i], L);
+    }
+    L = block_sum(L, scratch);                           // (a barrier: the weights are there)
+    if (p.sink) L += exp2f(p.sink[head] * 1.4426950408889634f - M + 15.f);
     const float inv = L != 0.f ? 1.0f / L : 0.f;
+    const int width = dv / 4, groups = MERGE_THREADS / width, group = threadIdx.x / width, d = threadIdx.x % width * 4;
+    const int share = (n + groups - 1) / groups, from = group * share, end = group < groups ? min(n, from + share) : from;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     constexpr int AHEAD = 8;
-    for (int d = threadIdx.x; d < dv; d += blockDim.x) {
-        float acc = 0.f;
-        for (int i0 = 0; i0 < n; i0 += AHEAD) {
-            float v[AHEAD];
+    for (int i0 = from; i0 < end; i0 += AHEAD) {
+        float4 v[AHEAD];
 #pragma unroll
-            for (int u = 0; u < AHEAD; ++u) v[u] = i0 + u < n ? part(i0 + u)[d] : 0.f;
+        for (int u = 0; u < AHEAD; ++u)
+            if (i0 + u < end) v[u] = *reinterpret_cast<const float4*>(p.partial + (cell + split(i0 + u)) * dv + d);
 #pragma unroll
-            for (int u = 0; u < AHEAD; ++u)
-                if (i0 + u < n) acc = fmaf(v[u], s_all[i0 + u], acc);
+        for (int u = 0; u < AHEAD; ++u)
+            if (i0 + u < end) {
+                const float w = s_w[i0 + u];
+                o.x = fmaf(v[u].x, w, o.x); o.y = fmaf(v[u].y, w, o.y); o.z = fmaf(v[u].z, w, o.z); o.w = fmaf(v[u].w, w, o.w);
+            }
+    }
+    s_o[threadIdx.x] = o;
+    __syncthreads();
+    if (group == 0) {
+        for (int i = 1; i < groups && i * share < n; ++i) {
+            const float4 v = s_o[i * width + threadIdx.x];
+            o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
         }
-        store_from_f32(p.out, p.out_f32 ? QS_F32 : QS_BF16, to + d, acc * inv);
+        store_from_f32(p.out, type, to + d, o.x * inv);
+        store_from_f32(p.out, type, to + d + 1, o.y * inv);
+        store_from_f32(p.out, type, to + d + 2, o.z * inv);
+        store_from_f32(p.out, type, to + d + 3, o.w * inv);
     }
 }
 
-// Keys of a block: four pages, two where they are wide (a block's pages then fill half of the shared memory of an SM as before).
-int split_keys(int dk, int dv) { return dk > 128 || dv > 128 ? 2 * PAGE : 4 * PAGE; }
+// Keys of a block: 256, half as many where they are wide (a block's keys and values then fill as much shared memory as before).
+int split_keys(int dk, int dv) { return WARPS * (dk > 128 || dv > 128 ? 16 : 32); }
 
-template <typename T, int KC, int VB, int WARPS>
+template <typename T, int KC, int VB, int KEYS>
 int go(const DecodeArgs& p, int rows, cudaStream_t stream) {
     constexpr int HEADS = sizeof(T) == 4 ? 4 : 8;
-    const int pages = WARPS * (PAGE * (p.dk + p.dv) + 128), sums = WARPS * HEADS * p.dv * 4, smem = pages > sums ? pages : sums;
+    const int pages = WARPS * (KEYS * (p.dk + p.dv) + 128), sums = WARPS * HEADS * p.dv * 4, smem = pages > sums ? pages : sums;
     static PerDevice limit;
     int device = 0;
     cudaGetDevice(&device);
-    limit.get(device, [] { return cudaFuncSetAttribute(kv8_decode_kernel<T, KC, VB, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024) == cudaSuccess ? 1 : 0; });
+    limit.get(device, [] { return cudaFuncSetAttribute(kv8_decode_kernel<T, KC, VB, KEYS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024) == cudaSuccess ? 1 : 0; });
     const int per = p.n_heads / p.n_kv_heads;
-    cudaError_t e = qs_launch_dependent(kv8_decode_kernel<T, KC, VB, WARPS>, dim3(p.splits, p.n_kv_heads * ((per + HEADS - 1) / HEADS), rows), dim3(WARPS * 32), (size_t)smem, stream, p);
+    cudaError_t e = qs_launch_dependent(kv8_decode_kernel<T, KC, VB, KEYS>, dim3(p.splits, p.n_kv_heads * ((per + HEADS - 1) / HEADS), rows), dim3(WARPS * 32), (size_t)smem, stream, p);
     if (e == cudaSuccess && p.splits > 1)
-        e = qs_launch_dependent(kv8_merge_kernel<WARPS * PAGE>, dim3(p.n_heads, rows), dim3(p.dv > 64 ? 128 : 64), (size_t)2 * p.splits * sizeof(float), stream, p);
+        e = qs_launch_dependent(kv8_merge_kernel<WARPS * KEYS>, dim3(p.n_heads, rows), dim3(MERGE_THREADS), (size_t)p.splits * sizeof(float), stream, p);
     if (e != cudaSuccess) return qs_fail(QS_ERR_INTERNAL, "kv8 decode: %s", cudaGetErrorString(e));
     return qs_check_launch("kv8 decode");
 }
@@ -393,7 +441,7 @@ int go(const DecodeArgs& p, int rows, cudaStream_t stream) {
 QS_API int qs_kv8_decode_splits(int dk, int dv, int max_context) { return (max_context + split_keys(dk, dv) - 1) / split_keys(dk, dv); }
 
 // out [T, n_heads * dv] (bfloat16, or float32 with out_f32), q [T, n_heads * dk] of type `dtype`; head sizes multiples of 16 up to 256.  `partial`: float32
-// [T][n_heads][splits][dv + 2] with qs_kv8_decode_splits(dk, dv, max_context) splits; contents need no initialisation; may be null for one split.
+// [T][n_heads][splits][dv + 2] with qs_kv8_decode_splits(dk, dv, max_context) splits, 16-byte aligned; contents need no initialisation; may be null for one split.
 // Masks, status codes and rows as for qs_kv8_attention; positions lie below max_context rounded up to whole splits.
 QS_API int qs_kv8_decode(void* out, int out_f32, long long ldo, const void* q, int dtype, long long ldq, int T_tokens, const int32_t* tok_slot,
                          const int32_t* tok_pos, const int32_t* page_table, int n_slots, int max_pages, int n_pages, const int8_t* k_cache,
@@ -410,11 +458,15 @@ QS_API int qs_kv8_decode(void* out, int out_f32, long long ldo, const void* q, i
     const int splits = qs_kv8_decode_splits(dk, dv, max_context);
     QS_REQUIRE(splits <= 4096, "kv8 decode: a context of %d exceeds what the merge holds (%d)", max_context, 4096 * split_keys(dk, dv));
     QS_REQUIRE(splits == 1 || partial, "kv8 decode: no workspace");
-    const DecodeArgs p = {out, partial, q, k_cache, v_cache, k_scale, v_scale, sink, tok_slot, tok_pos, page_table, (size_t)ldo, (size_t)ldq,
-                          max_pages, n_slots, n_pages, n_heads, n_kv_heads, dk, dv, window, chunk, keep_first, splits, out_f32, scale, softcap, status};
-#define GO(T) do { if (dk <= 64 && dv <= 128) return go<T, 1, 1, 4>(p, T_tokens, stream); \
-                   if (dk <= 128 && dv <= 128) return go<T, 2, 1, 4>(p, T_tokens, stream); \
-                   return go<T, 4, 2, 2>(p, T_tokens, stream); } while (0)
+    QS_REQUIRE(((uintptr_t)partial % 16) == 0, "kv8 decode: the workspace must be 16-byte aligned");
+    const int e = dtype == QS_F32 ? 4 : 2;
+    const int q_aligned = ((uintptr_t)q % 16) == 0 && ldq * e % 16 == 0;
+    const DecodeArgs p = {out, partial, (float2*)(partial + (size_t)T_tokens * n_heads * splits * dv), q, k_cache, v_cache, k_scale, v_scale, sink, tok_slot, tok_pos, page_table, (size_t)ldo, (size_t)ldq,
+                          max_pages, n_slots, n_pages, n_heads, n_kv_heads, dk, dv, window, chunk, keep_first, splits, out_f32, scale, softcap,
+                          softcap > 0.f ? 2.f * 1.4426950408889634f / softcap : 0.f, q_aligned, status};
+#define GO(T) do { if (dk <= 64 && dv <= 128) return go<T, 1, 1, 32>(p, T_tokens, stream); \
+                   if (dk <= 128 && dv <= 128) return go<T, 2, 1, 32>(p, T_tokens, stream); \
+                   return go<T, 4, 2, 16>(p, T_tokens, stream); } while (0)
     if (dtype == QS_F32) GO(float);
     GO(__nv_bfloat16);
 #undef GO
