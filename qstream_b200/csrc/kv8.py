@@ -18,11 +18,11 @@ from .q4 import TYPES, _on_current_device, _refuse
 PAGE_TOKENS = 64
 MAX_SPLIT_CONTEXT = 4096 * 128      # what the merge of the keys' parts holds for any head size; longer contexts go a row at a time
 
-_store = _read = _attention = _decode = _splits = None
+_store = _read = _attention = _decode = _scratch = None
 
 
 def _bind():
-    global _store, _read, _attention, _decode, _splits
+    global _store, _read, _attention, _decode, _scratch
     if _store is None:
         _read = ops.bind("qs_kv8_read_pages", [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p])
         _attention = ops.bind("qs_kv8_attention", [
@@ -31,7 +31,7 @@ def _bind():
         _decode = ops.bind("qs_kv8_decode", [
             c_void_p, c_int, c_longlong, c_void_p, c_int, c_longlong, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
             c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p, c_float, c_int, c_void_p, c_void_p, c_void_p])
-        _splits = ops.bind("qs_kv8_decode_splits", [c_int, c_int, c_int])
+        _scratch = ops.bind("qs_kv8_decode_scratch", [c_int, c_int, c_int, c_int, c_int], c_longlong)
         _store = ops.bind("qs_kv8_store", [
             c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong, c_float, c_int,
             c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
@@ -172,8 +172,8 @@ def decode(q, n_heads, n_kv_heads, head_dim, scale, window, tok_slot, tok_pos, p
     ops.ptr(q)
     _bind()
     if head_dim % 16 == 0 and dv % 16 == 0 and head_dim <= 256 and dv <= 256 and T <= 65535 and max_context <= MAX_SPLIT_CONTEXT:
-        splits = _splits(head_dim, dv, max_context)
-        partial = torch.empty((T * n_heads * splits * (dv + 2),), dtype=torch.float32, device=q.device) if splits > 1 else None
+        floats = _scratch(T, n_heads, head_dim, dv, max_context)
+        partial = torch.empty((floats,), dtype=torch.float32, device=q.device) if floats else None
         ops.check(_decode(ops.ptr(out), int(out.dtype == torch.float32), out.stride(0), ops.ptr(q), ops.dtype_code(q), q.stride(0), T, ops.ptr(tok_slot), ops.ptr(tok_pos),
                           ops.ptr(page_table), page_table.shape[0], page_table.shape[1], k_cache.shape[0], ops.ptr(k_cache), ops.ptr(v_cache), ops.ptr(k_scale),
                           ops.ptr(v_scale), n_heads, n_kv_heads, head_dim, dv, float(scale), int(window), int(chunk), int(keep_first), ops.ptr(sink),

@@ -2,9 +2,9 @@
 //
 //   s[u] = scale * q.K[u] (capped), K[u] = code * scale of u's page;  softmax over the keys that the mask leaves;  o = sum_u p[u] V[u]
 //
-// Bound by the bytes of the pages.  A warp takes 32 keys (16 of wide heads) and up to HEADS query heads that share their key head: two
-// bulk copies bring keys and values into shared memory (all of a block are on their way at once, from the first instructions on),
-// 16-bit products on mma.m16n8k16 take them from there.
+// Bound by the bytes of the pages.  A warp takes 32 keys (16 of wide heads) and up to HEADS query heads that share their key head: a bulk
+// copy brings the keys into shared memory, asynchronous copies the values, their rows apart (all of a block are on their way at once, from
+// the first instructions on); 16-bit products on mma.m16n8k16 take them from there.
 //
 //   scores   left operand: 16 keys, right: the heads.  A lane's 16 bytes of a key's row are its part of four steps; which dims meet in
 //            a step is free, so the queries are laid out the same way.  A code, as the low byte of a 16-bit float 1024 beside its upper
@@ -32,7 +32,7 @@ constexpr int PAGE = 64, WARPS = 8;
 
 struct DecodeArgs {
     void* out;
-    float* partial;                                      // [rows][heads][splits][dv]
+    float* partial;                                      // [rows][heads][splits][places]
     float2* ml;                                          // [rows][heads][splits]: maximum (base two), sum
     const void* q;
     const int8_t *k_cache, *v_cache;
@@ -91,21 +91,33 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                  ::"r"(sm100::smem_u32(dst)), "l"(src), "r"(bytes), "r"(sm100::smem_u32(bar)) : "memory");
 }
 
-// KC: blocks of 64 dims that keys span at most; VB: blocks of 128 dims of the values; a warp takes KEYS keys.
-template <typename T, int KC, int VB, int KEYS>
+// Four neighbouring places of a head's sums: dims d, d + 1 and d + 16, d + 17.
+__device__ __forceinline__ int dim_of(int place) { return (place & ~127) + 8 * (place & 15) - 7 * (place & 1) + 2 * (place >> 4 & 7); }
+__device__ __forceinline__ void store_places(void* out, int type, size_t at, float4 o, float factor, bool both) {
+    store_from_f32(out, type, at, o.x * factor);
+    store_from_f32(out, type, at + 1, o.y * factor);
+    if (both) {
+        store_from_f32(out, type, at + 16, o.z * factor);
+        store_from_f32(out, type, at + 17, o.w * factor);
+    }
+}
+
+// KC: blocks of 64 dims that keys span at most; VB: blocks of 128 dims of the values; a warp takes KEYS keys.  FULL: keys and values fill the
+// blocks (addresses are then constants apart).
+template <typename T, int KC, int VB, int KEYS, bool FULL>
 __global__ void __launch_bounds__(WARPS * 32)
 kv8_decode_kernel(const DecodeArgs p) {
     constexpr bool WIDE = sizeof(T) == 4;                // two columns to a head
     constexpr int HEADS = WIDE ? 4 : 8, SPLIT = WARPS * KEYS, TILES = KEYS / 16;
+    const int dk = FULL ? KC * 64 : p.dk, dv = FULL ? VB * 128 : p.dv;
     extern __shared__ __align__(128) uint8_t smem[];     // per warp: its keys, its values; in the end [WARPS][HEADS][dv] sums
-    __shared__ uint64_t bars[WARPS][2];
+    __shared__ uint64_t bar[WARPS];
     __shared__ float s_m[WARPS][HEADS], s_l[WARPS][HEADS], s_unit[8];
     __shared__ uint32_t s_q[KC * 8][32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     grid_dep_launch();
     if (lane == 0) {
-        sm100::mbar_init(&bars[warp][0], 1);
-        sm100::mbar_init(&bars[warp][1], 1);
+        sm100::mbar_init(&bar[warp], 1);
         sm100::mbar_fence_init();
         sm100::fence_proxy_async_smem();
     }
@@ -115,10 +127,21 @@ kv8_decode_kernel(const DecodeArgs p) {
     const int split = blockIdx.x, kvh = blockIdx.y / head_tiles, row = blockIdx.z;
     const int head0 = kvh * per + blockIdx.y % head_tiles * HEADS, heads = min(HEADS, per - blockIdx.y % head_tiles * HEADS);
     const int slot = p.tok_slot[row], pos = p.tok_pos[row];
+    // The queries, laid out for all warps: warp w makes column w, which is head w (WIDE: head w & 3, its first or second term); lane l
+    // its dims 8 l .. 8 l + 7.  A lane of the products has dims 64 c + 16 t .. + 15 of column g.  Their way from memory runs beside that of the step's metadata.
+    float x[8];
+    {
+        const T* src = reinterpret_cast<const T*>(p.q) + (size_t)row * p.ldq + (size_t)(head0 + min(WIDE ? warp & 3 : warp, heads - 1)) * dk + 8 * lane;
+        if (8 * lane < dk && p.q_aligned) load8_as_f32(src, WIDE ? QS_F32 : QS_BF16, 0, x);
+        else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = 8 * lane + i < dk ? to_f32(src[i]) : 0.f;
+        }
+    }
     if (slot < 0 || slot >= p.n_slots || pos < 0 || (pos >> 6) >= p.max_pages || pos >= p.splits * SPLIT) {
         if (slot >= 0 && threadIdx.x == 0 && split == 0 && blockIdx.y == 0) atomicExch(p.status, 1);
         if (p.splits == 1)                               // no merge: the row's zeros are written here
-            for (int i = threadIdx.x; i < heads * p.dv; i += WARPS * 32) store_from_f32(p.out, p.out_f32 ? QS_F32 : QS_BF16, (size_t)row * p.ldo + (size_t)head0 * p.dv + i, 0.f);
+            for (int i = threadIdx.x; i < heads * dv; i += WARPS * 32) store_from_f32(p.out, p.out_f32 ? QS_F32 : QS_BF16, (size_t)row * p.ldo + (size_t)head0 * dv + i, 0.f);
         return;
     }
     const int first = first_key(p, pos), keep = p.window > 0 ? min(p.keep_first, first) : 0;
@@ -131,30 +154,32 @@ kv8_decode_kernel(const DecodeArgs p) {
         page = p.page_table[(size_t)slot * p.max_pages + (key0 >> 6)];
         if (page < 0 || page >= p.n_pages) { if (lane == 0) atomicExch(p.status, 3); page = -1; }
     }
-    const int warp_bytes = KEYS * (p.dk + p.dv) + 128;   // rows are read in whole blocks of dims: up to 127 bytes beyond the last
+    // Rows are read in whole blocks of dims: up to 127 bytes beyond the last.  Values lie 16 bytes more than a row apart: the rows of a lane's
+    // keys then meet other banks than its neighbours' (64 bytes of two banks' rows otherwise, a quarter of the rate).
+    const int pitch = dv + 16, warp_bytes = KEYS * (dk + pitch) + 128;
     uint8_t* keys = smem + warp * warp_bytes;
-    uint8_t* values = keys + KEYS * p.dk;
+    uint8_t* values = keys + KEYS * dk;
     const size_t at = (size_t)max(page, 0) * p.n_kv_heads + kvh;
-    if (page >= 0 && lane == 0) {
+    if (page >= 0) {
         const int n = min(KEYS, pos - key0 + 1);         // rows behind the sequence's end stay out of it
         const size_t in_page = at * PAGE + (key0 & (PAGE - 1));
-        sm100::mbar_expect_tx(&bars[warp][0], n * p.dk);
-        bulk_load(keys, p.k_cache + in_page * p.dk, n * p.dk, &bars[warp][0]);
-        sm100::mbar_expect_tx(&bars[warp][1], n * p.dv);
-        bulk_load(values, p.v_cache + in_page * p.dv, n * p.dv, &bars[warp][1]);
-    }
-    const float ks = page >= 0 ? p.k_scale[at] : 0.f, vs = page >= 0 ? p.v_scale[at] : 0.f;
-
-    // The queries, laid out for all warps: warp w makes column w, which is head w (WIDE: head w & 3, its first or second term); lane l
-    // its dims 8 l .. 8 l + 7.  A lane of the products has dims 64 c + 16 t .. + 15 of column g.
-    {
-        const T* src = reinterpret_cast<const T*>(p.q) + (size_t)row * p.ldq + (size_t)(head0 + min(WIDE ? warp & 3 : warp, heads - 1)) * p.dk + 8 * lane;
-        float x[8];
-        if (8 * lane < p.dk && p.q_aligned) load8_as_f32(src, WIDE ? QS_F32 : QS_BF16, 0, x);
-        else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = 8 * lane + i < p.dk ? to_f32(src[i]) : 0.f;
+        if (lane == 0) {
+            sm100::mbar_expect_tx(&bar[warp], n * dk);
+            bulk_load(keys, p.k_cache + in_page * dk, n * dk, &bar[warp]);
         }
+        const int pieces = dv >> 4;                      // 16 bytes of a row to a lane
+        for (int i = lane; i < n * pieces; i += 32) {
+            const int r = i / pieces, c = i - r * pieces;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(sm100::smem_u32(values + r * pitch + 16 * c)), "l"(p.v_cache + (in_page + r) * dv + 16 * c) : "memory");
+        }
+    }
+    float ks = 0.f, vs = 0.f;                            // no page: sums of 0, times 0
+    if (page >= 0) {                                     // here, not where they are used: their way from memory is long
+        asm volatile("ld.global.f32 %0, [%1];" : "=f"(ks) : "l"(p.k_scale + at));
+        asm volatile("ld.global.f32 %0, [%1];" : "=f"(vs) : "l"(p.v_scale + at));
+    }
+
+    {
         float most = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[i]));
@@ -182,7 +207,7 @@ kv8_decode_kernel(const DecodeArgs p) {
     float acc[VB * 8][4];
 #pragma unroll
     for (int j = 0; j < VB * 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-    const bool ok = page >= 0 && sm100::mbar_wait(&bars[warp][0], 0);
+    const bool ok = page >= 0 && sm100::mbar_wait(&bar[warp], 0);
     if (page >= 0 && !ok && lane == 0) atomicExch(p.status, 123);
     if (ok) {
         // scores of the keys: tile i, row g (and g + 8) is key 16 i + g (+ 8)
@@ -192,14 +217,14 @@ kv8_decode_kernel(const DecodeArgs p) {
         for (int i = 0; i < TILES; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
 #pragma unroll
         for (int c = 0; c < KC; ++c) {
-            if (64 * c >= p.dk) break;
+            if (64 * c >= dk) break;
             uint32_t qf[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) qf[i] = s_q[c * 8 + i][lane];
 #pragma unroll
             for (int i = 0; i < TILES; ++i) {
-                const uint4 lo = *reinterpret_cast<const uint4*>(keys + (16 * i + g) * p.dk + 64 * c + 16 * t);
-                const uint4 hi = *reinterpret_cast<const uint4*>(keys + (16 * i + g + 8) * p.dk + 64 * c + 16 * t);
+                const uint4 lo = *reinterpret_cast<const uint4*>(keys + (16 * i + g) * dk + 64 * c + 16 * t);
+                const uint4 hi = *reinterpret_cast<const uint4*>(keys + (16 * i + g + 8) * dk + 64 * c + 16 * t);
                 const uint32_t a[4] = {lo.x ^ 0x80808080u, lo.y ^ 0x80808080u, lo.z ^ 0x80808080u, lo.w ^ 0x80808080u};
                 const uint32_t b[4] = {hi.x ^ 0x80808080u, hi.y ^ 0x80808080u, hi.z ^ 0x80808080u, hi.w ^ 0x80808080u};
 #pragma unroll
@@ -208,25 +233,35 @@ kv8_decode_kernel(const DecodeArgs p) {
             }
         }
         const bool whole = key0 + KEYS - 1 <= pos && (key0 >= first || key0 + KEYS <= keep);
+        const float factor[2] = {p.softcap > 0.f ? unit[0] : unit[0] * log2e, p.softcap > 0.f ? unit[1] : unit[1] * log2e};
 #pragma unroll
         for (int i = 0; i < TILES; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                float x = s[i][e];
-                if (WIDE) x += __shfl_xor_sync(0xffffffffu, x, 2);
-                x *= unit[e & 1];
-                if (p.softcap > 0.f) {
-                    if (WIDE) x = p.softcap * tanhf(x / p.softcap);
-                    else x = p.softcap - __fdividef(2.f * p.softcap, fast_exp2(x * p.cap_k2) + 1.f);      // tanh u = 1 - 2 / (e^2u + 1), within 10^-6 of the cap
-                }
-                x *= log2e;
-                if (!whole) {
-                    const int key = key0 + 16 * i + g + 8 * (e >> 1);
-                    if (key > pos || (key < first && key >= keep)) x = -INFINITY;
-                }
-                s[i][e] = x;
-                m[e & 1] = fmaxf(m[e & 1], x);
+                if (WIDE) s[i][e] += __shfl_xor_sync(0xffffffffu, s[i][e], 2);
+                s[i][e] *= factor[e & 1];
             }
+        if (p.softcap > 0.f) {
+            const float cap = p.softcap * log2e;
+#pragma unroll
+            for (int i = 0; i < TILES; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)              // tanh u = 1 - 2 / (e^2u + 1), within 10^-6 of the cap
+                    s[i][e] = WIDE ? cap * tanhf(s[i][e] / p.softcap) : cap - __fdividef(2.f * cap, fast_exp2(s[i][e] * p.cap_k2) + 1.f);
+        }
+        if (!whole) {
+#pragma unroll
+            for (int i = 0; i < TILES; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int key = key0 + 16 * i + g + 8 * (e >> 1);
+                    if (key > pos || (key < first && key >= keep)) s[i][e] = -INFINITY;
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < TILES; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) m[e & 1] = fmaxf(m[e & 1], s[i][e]);
         // the weights, in pairs of heads; the columns' maxima and sums over the eight lanes of a column
         uint32_t w[TILES][2];                            // tile i, rows g and g + 8: two heads
 #pragma unroll
@@ -252,94 +287,92 @@ kv8_decode_kernel(const DecodeArgs p) {
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) l[j] += __shfl_xor_sync(0xffffffffu, l[j], o);
-        if (sm100::mbar_wait(&bars[warp][1], 0)) {
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncwarp();
 #pragma unroll
-            for (int i = 0; i < TILES; ++i)              // 16 keys: this lane's are 2 t, 2 t + 1 and the same + 8
+        for (int i = 0; i < TILES; ++i)              // 16 keys: this lane's are 2 t, 2 t + 1 and the same + 8
 #pragma unroll
-                for (int b = 0; b < VB; ++b) {
-                    if (128 * b >= p.dv) break;
-                    const uint8_t* v = values + (16 * i + 2 * t) * p.dv + 128 * b + 16 * g;
-                    uint4 x[4];
+            for (int b = 0; b < VB; ++b) {
+                if (128 * b >= dv) break;
+                const uint8_t* v = values + (16 * i + 2 * t) * pitch + 128 * b + 16 * g;
+                uint4 x[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        x[e] = *reinterpret_cast<const uint4*>(v + ((e & 1) + 8 * (e >> 1)) * p.dv);
-                        x[e].x ^= 0x80808080u; x[e].y ^= 0x80808080u; x[e].z ^= 0x80808080u; x[e].w ^= 0x80808080u;
-                    }
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {        // four dims: tiles 2 k and 2 k + 1
-                        const uint32_t x0 = k == 0 ? x[0].x : k == 1 ? x[0].y : k == 2 ? x[0].z : x[0].w, x1 = k == 0 ? x[1].x : k == 1 ? x[1].y : k == 2 ? x[1].z : x[1].w;
-                        const uint32_t x2 = k == 0 ? x[2].x : k == 1 ? x[2].y : k == 2 ? x[2].z : x[2].w, x3 = k == 0 ? x[3].x : k == 1 ? x[3].y : k == 2 ? x[3].z : x[3].w;
-                        const uint32_t n0 = __byte_perm(x0, x1, 0x5140), n1 = __byte_perm(x0, x1, 0x7362), f0 = __byte_perm(x2, x3, 0x5140), f1 = __byte_perm(x2, x3, 0x7362);
-                        mma_sum<WIDE>(acc[8 * b + 2 * k], two_codes(n0, 0x4140), two_codes(n0, 0x4342), two_codes(f0, 0x4140), two_codes(f0, 0x4342), w[i][0], w[i][1]);
-                        mma_sum<WIDE>(acc[8 * b + 2 * k + 1], two_codes(n1, 0x4140), two_codes(n1, 0x4342), two_codes(f1, 0x4140), two_codes(f1, 0x4342), w[i][0], w[i][1]);
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    x[e] = *reinterpret_cast<const uint4*>(v + ((e & 1) + 8 * (e >> 1)) * pitch);
+                    x[e].x ^= 0x80808080u; x[e].y ^= 0x80808080u; x[e].z ^= 0x80808080u; x[e].w ^= 0x80808080u;
                 }
-        } else if (lane == 0) {
-            atomicExch(p.status, 124);
-        }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {        // four dims: tiles 2 k and 2 k + 1
+                    const uint32_t x0 = k == 0 ? x[0].x : k == 1 ? x[0].y : k == 2 ? x[0].z : x[0].w, x1 = k == 0 ? x[1].x : k == 1 ? x[1].y : k == 2 ? x[1].z : x[1].w;
+                    const uint32_t x2 = k == 0 ? x[2].x : k == 1 ? x[2].y : k == 2 ? x[2].z : x[2].w, x3 = k == 0 ? x[3].x : k == 1 ? x[3].y : k == 2 ? x[3].z : x[3].w;
+                    const uint32_t n0 = __byte_perm(x0, x1, 0x5140), n1 = __byte_perm(x0, x1, 0x7362), f0 = __byte_perm(x2, x3, 0x5140), f1 = __byte_perm(x2, x3, 0x7362);
+                    mma_sum<WIDE>(acc[8 * b + 2 * k], two_codes(n0, 0x4140), two_codes(n0, 0x4342), two_codes(f0, 0x4140), two_codes(f0, 0x4342), w[i][0], w[i][1]);
+                    mma_sum<WIDE>(acc[8 * b + 2 * k + 1], two_codes(n1, 0x4140), two_codes(n1, 0x4342), two_codes(f1, 0x4140), two_codes(f1, 0x4342), w[i][0], w[i][1]);
+                }
+            }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");     // (a wait for the keys that ran out: the values' copies end before their place is used again)
     // The warps' results: sums as [head][dim], beside each other where the pages were.
-    if (g == 0 && (!WIDE || t < 2)) { s_m[warp][h0] = m[0]; s_m[warp][h0 + 1] = m[1]; s_l[warp][h0] = l[0]; s_l[warp][h0 + 1] = l[1]; }
+    if (g == 0 && (!WIDE || t < 2)) { s_m[warp][h0] = m[0]; s_m[warp][h0 + 1] = m[1]; }
     __syncthreads();                                     // everybody has read its keys and values
+    // [warp][head][tile j][row g, row g + 8]: place 16 j + 2 g + e is dim 16 g + 2 j + e (of each 128); four floats more to a head, and the lanes' pairs meet all banks
+    constexpr int PLACES = VB * 128, PITCH = PLACES + 4;
     float* sums = reinterpret_cast<float*>(smem);
     // what a warp's sums count beside the others'; a warp without a key that is seen: nothing; one whose scores are all NaN: NaN
-    float M[2] = {-INFINITY, -INFINITY}, a[2];
+    float f[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
+        float M = s_m[0][h0 + j];
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) M[j] = fmaxf(M[j], s_m[w][h0 + j]);
-        a[j] = (m[j] == -INFINITY ? 1.f : exp2f(m[j] - M[j]));
+        for (int w = 1; w < WARPS; ++w) M = fmaxf(M, s_m[w][h0 + j]);
+        f[j] = m[j] == -INFINITY ? 1.f : fast_exp2(m[j] - M);
+        if (g == 0 && (!WIDE || t < 2)) {
+            s_l[warp][h0 + j] = l[j] * f[j];
+            if (warp == 0) s_unit[h0 + j] = M;
+        }
+        f[j] *= vs;
     }
 #pragma unroll
     for (int j = 0; j < VB * 8; ++j) {
         const int d = (j >> 3) * 128 + 16 * g + 2 * (j & 7);
+        if (WIDE) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (WIDE) acc[j][e] += __shfl_xor_sync(0xffffffffu, acc[j][e], 2);
-            acc[j][e] = page >= 0 ? acc[j][e] * vs * a[e & 1] : 0.f;
+            for (int e = 0; e < 4; ++e) acc[j][e] += __shfl_xor_sync(0xffffffffu, acc[j][e], 2);
         }
-        if (d < p.dv && (!WIDE || t < 2)) {
-            if (h0 < heads) *reinterpret_cast<float2*>(sums + (warp * HEADS + h0) * p.dv + d) = make_float2(acc[j][0], acc[j][2]);
-            if (h0 + 1 < heads) *reinterpret_cast<float2*>(sums + (warp * HEADS + h0 + 1) * p.dv + d) = make_float2(acc[j][1], acc[j][3]);
+        if (d < dv && (!WIDE || t < 2)) {
+            float* to = sums + (warp * HEADS + h0) * PITCH + 16 * j + 2 * g;
+            if (h0 < heads) *reinterpret_cast<float2*>(to) = make_float2(acc[j][0] * f[0], acc[j][2] * f[0]);
+            if (h0 + 1 < heads) *reinterpret_cast<float2*>(to + PITCH) = make_float2(acc[j][1] * f[1], acc[j][3] * f[1]);
         }
     }
     __syncthreads();
-    if (warp < heads) {                                  // a head to a warp
-        for (int h = warp; h < heads; h += WARPS) {
-            float Mh = -INFINITY, L = 0.f;
+    for (int i = 4 * threadIdx.x; i < heads * PLACES; i += 4 * WARPS * 32) {
+        const int h = i / PLACES, place = i % PLACES, d = dim_of(place);
+        if (d >= dv) continue;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        float L = 0.f;
 #pragma unroll
-            for (int w = 0; w < WARPS; ++w) Mh = fmaxf(Mh, s_m[w][h]);
-#pragma unroll
-            for (int w = 0; w < WARPS; ++w) L = fmaf(s_l[w][h], s_m[w][h] == -INFINITY ? 1.f : exp2f(s_m[w][h] - Mh), L);
-            float factor = 1.f;
-            if (p.splits == 1) {                         // as the merge of one split
-                if (p.sink) {
-                    const float sink = p.sink[head0 + h] * 1.4426950408889634f, all = fmaxf(Mh, sink);
-                    factor = Mh == -INFINITY ? 1.f : exp2f(Mh - all);
-                    L = fmaf(L, factor, exp2f(sink - all + 15.f));
-                }
-                factor *= L != 0.f ? 1.0f / L : 0.f;
-            }
+        for (int w = 0; w < WARPS; ++w) {
+            const float4 v = *reinterpret_cast<const float4*>(sums + (w * HEADS + h) * PITCH + place);
+            o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
+            L += s_l[w][h];
+        }
+        if (p.splits > 1) {
             const size_t cell = ((size_t)row * p.n_heads + head0 + h) * p.splits + split;
-            for (int d = 4 * lane; d < p.dv; d += 128) {
-                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-                for (int w = 0; w < WARPS; ++w) {
-                    const float4 v = *reinterpret_cast<const float4*>(sums + (w * HEADS + h) * p.dv + d);
-                    o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
-                }
-                if (p.splits > 1) {
-                    *reinterpret_cast<float4*>(p.partial + cell * p.dv + d) = o;
-                } else {
-                    const size_t to = (size_t)row * p.ldo + (size_t)(head0 + h) * p.dv + d;
-                    const int type = p.out_f32 ? QS_F32 : QS_BF16;
-                    store_from_f32(p.out, type, to, o.x * factor);
-                    store_from_f32(p.out, type, to + 1, o.y * factor);
-                    store_from_f32(p.out, type, to + 2, o.z * factor);
-                    store_from_f32(p.out, type, to + 3, o.w * factor);
-                }
+            *reinterpret_cast<float4*>(p.partial + cell * PLACES + place) = o;
+            if (place == 0) p.ml[cell] = make_float2(s_unit[h], L);
+        } else {                                         // as the merge of one split
+            const float M = s_unit[h];
+            float factor = 1.f;
+            if (p.sink) {
+                const float sink = p.sink[head0 + h] * 1.4426950408889634f, all = fmaxf(M, sink);
+                factor = M == -INFINITY ? 1.f : exp2f(M - all);
+                L = fmaf(L, factor, exp2f(sink - all + 15.f));
             }
-            if (p.splits > 1 && lane == 0) p.ml[cell] = make_float2(Mh, L);
+            factor *= L != 0.f ? 1.0f / L : 0.f;
+            const size_t to = (size_t)row * p.ldo + (size_t)(head0 + h) * dv + d;
+            const int type = p.out_f32 ? QS_F32 : QS_BF16;
+            store_places(p.out, type, to, o, factor, d + 16 < dv);
         }
     }
 }
@@ -347,7 +380,7 @@ kv8_decode_kernel(const DecodeArgs p) {
 // One block per row and head: the splits' results.  The threads of a group have four dims each; the groups share the splits, each in
 // ascending order, and are added in theirs; how the splits are shared depends on their number for the row and on dv.
 constexpr int MERGE_THREADS = 256;
-template <int SPLIT>
+template <int SPLIT, int PLACES>
 __global__ void __launch_bounds__(MERGE_THREADS)
 kv8_merge_kernel(const DecodeArgs p) {
     extern __shared__ float s_w[];                       // [splits] weights
@@ -386,15 +419,16 @@ kv8_merge_kernel(const DecodeArgs p) {
     L = block_sum(L, scratch);                           // (a barrier: the weights are there)
     if (p.sink) L += exp2f(p.sink[head] * 1.4426950408889634f - M + 15.f);
     const float inv = L != 0.f ? 1.0f / L : 0.f;
-    const int width = dv / 4, groups = MERGE_THREADS / width, group = threadIdx.x / width, d = threadIdx.x % width * 4;
-    const int share = (n + groups - 1) / groups, from = group * share, end = group < groups ? min(n, from + share) : from;
+    constexpr int width = PLACES / 4, groups = MERGE_THREADS / width;
+    const int group = threadIdx.x / width, place = threadIdx.x % width * 4, d = dim_of(place);
+    const int share = (n + groups - 1) / groups, from = group * share, end = d < dv ? min(n, from + share) : from;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     constexpr int AHEAD = 8;
     for (int i0 = from; i0 < end; i0 += AHEAD) {
         float4 v[AHEAD];
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u)
-            if (i0 + u < end) v[u] = *reinterpret_cast<const float4*>(p.partial + (cell + split(i0 + u)) * dv + d);
+            if (i0 + u < end) v[u] = *reinterpret_cast<const float4*>(p.partial + (cell + split(i0 + u)) * PLACES + place);
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u)
             if (i0 + u < end) {
@@ -404,44 +438,48 @@ kv8_merge_kernel(const DecodeArgs p) {
     }
     s_o[threadIdx.x] = o;
     __syncthreads();
-    if (group == 0) {
+    if (group == 0 && d < dv) {
         for (int i = 1; i < groups && i * share < n; ++i) {
             const float4 v = s_o[i * width + threadIdx.x];
             o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
         }
-        store_from_f32(p.out, type, to + d, o.x * inv);
-        store_from_f32(p.out, type, to + d + 1, o.y * inv);
-        store_from_f32(p.out, type, to + d + 2, o.z * inv);
-        store_from_f32(p.out, type, to + d + 3, o.w * inv);
+        store_places(p.out, type, to + d, o, inv, d + 16 < dv);
     }
 }
 
 // Keys of a block: 256, half as many where they are wide (a block's keys and values then fill as much shared memory as before).
 int split_keys(int dk, int dv) { return WARPS * (dk > 128 || dv > 128 ? 16 : 32); }
 
-template <typename T, int KC, int VB, int KEYS>
+// Places of a head's sums.
+int places(int dk, int dv) { return dk > 128 || dv > 128 ? 256 : 128; }
+
+template <typename T, int KC, int VB, int KEYS, bool FULL>
 int go(const DecodeArgs& p, int rows, cudaStream_t stream) {
     constexpr int HEADS = sizeof(T) == 4 ? 4 : 8;
-    const int pages = WARPS * (KEYS * (p.dk + p.dv) + 128), sums = WARPS * HEADS * p.dv * 4, smem = pages > sums ? pages : sums;
+    const int pages = WARPS * (KEYS * (p.dk + p.dv + 16) + 128), sums = WARPS * HEADS * (VB * 128 + 4) * 4, smem = pages > sums ? pages : sums;
     static PerDevice limit;
     int device = 0;
     cudaGetDevice(&device);
-    limit.get(device, [] { return cudaFuncSetAttribute(kv8_decode_kernel<T, KC, VB, KEYS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024) == cudaSuccess ? 1 : 0; });
+    limit.get(device, [] { return cudaFuncSetAttribute(kv8_decode_kernel<T, KC, VB, KEYS, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024) == cudaSuccess ? 1 : 0; });
     const int per = p.n_heads / p.n_kv_heads;
-    cudaError_t e = qs_launch_dependent(kv8_decode_kernel<T, KC, VB, KEYS>, dim3(p.splits, p.n_kv_heads * ((per + HEADS - 1) / HEADS), rows), dim3(WARPS * 32), (size_t)smem, stream, p);
+    cudaError_t e = qs_launch_dependent(kv8_decode_kernel<T, KC, VB, KEYS, FULL>, dim3(p.splits, p.n_kv_heads * ((per + HEADS - 1) / HEADS), rows), dim3(WARPS * 32), (size_t)smem, stream, p);
     if (e == cudaSuccess && p.splits > 1)
-        e = qs_launch_dependent(kv8_merge_kernel<WARPS * KEYS>, dim3(p.n_heads, rows), dim3(MERGE_THREADS), (size_t)p.splits * sizeof(float), stream, p);
+        e = qs_launch_dependent(kv8_merge_kernel<WARPS * KEYS, VB * 128>, dim3(p.n_heads, rows), dim3(MERGE_THREADS), (size_t)p.splits * sizeof(float), stream, p);
     if (e != cudaSuccess) return qs_fail(QS_ERR_INTERNAL, "kv8 decode: %s", cudaGetErrorString(e));
     return qs_check_launch("kv8 decode");
 }
 
 }  // namespace
 
-// Splits of the keys that a call is made for (1: no merge, no workspace).
+// Splits of the keys that a call is made for, and floats of workspace that it takes (0: one split, no merge).
 QS_API int qs_kv8_decode_splits(int dk, int dv, int max_context) { return (max_context + split_keys(dk, dv) - 1) / split_keys(dk, dv); }
+QS_API long long qs_kv8_decode_scratch(int T_tokens, int n_heads, int dk, int dv, int max_context) {
+    const int splits = qs_kv8_decode_splits(dk, dv, max_context);
+    return splits > 1 ? (long long)T_tokens * n_heads * splits * (places(dk, dv) + 2) : 0;
+}
 
-// out [T, n_heads * dv] (bfloat16, or float32 with out_f32), q [T, n_heads * dk] of type `dtype`; head sizes multiples of 16 up to 256.  `partial`: float32
-// [T][n_heads][splits][dv + 2] with qs_kv8_decode_splits(dk, dv, max_context) splits, 16-byte aligned; contents need no initialisation; may be null for one split.
+// out [T, n_heads * dv] (bfloat16, or float32 with out_f32), q [T, n_heads * dk] of type `dtype`; head sizes multiples of 16 up to 256.  `partial`: float32,
+// qs_kv8_decode_scratch elements, 16-byte aligned; contents need no initialisation; may be null for one split.
 // Masks, status codes and rows as for qs_kv8_attention; positions lie below max_context rounded up to whole splits.
 QS_API int qs_kv8_decode(void* out, int out_f32, long long ldo, const void* q, int dtype, long long ldq, int T_tokens, const int32_t* tok_slot,
                          const int32_t* tok_pos, const int32_t* page_table, int n_slots, int max_pages, int n_pages, const int8_t* k_cache,
@@ -461,12 +499,14 @@ QS_API int qs_kv8_decode(void* out, int out_f32, long long ldo, const void* q, i
     QS_REQUIRE(((uintptr_t)partial % 16) == 0, "kv8 decode: the workspace must be 16-byte aligned");
     const int e = dtype == QS_F32 ? 4 : 2;
     const int q_aligned = ((uintptr_t)q % 16) == 0 && ldq * e % 16 == 0;
-    const DecodeArgs p = {out, partial, (float2*)(partial + (size_t)T_tokens * n_heads * splits * dv), q, k_cache, v_cache, k_scale, v_scale, sink, tok_slot, tok_pos, page_table, (size_t)ldo, (size_t)ldq,
+    const DecodeArgs p = {out, partial, (float2*)(partial + (size_t)T_tokens * n_heads * splits * places(dk, dv)), q, k_cache, v_cache, k_scale, v_scale, sink, tok_slot, tok_pos, page_table, (size_t)ldo, (size_t)ldq,
                           max_pages, n_slots, n_pages, n_heads, n_kv_heads, dk, dv, window, chunk, keep_first, splits, out_f32, scale, softcap,
                           softcap > 0.f ? 2.f * 1.4426950408889634f / softcap : 0.f, q_aligned, status};
-#define GO(T) do { if (dk <= 64 && dv <= 128) return go<T, 1, 1, 32>(p, T_tokens, stream); \
-                   if (dk <= 128 && dv <= 128) return go<T, 2, 1, 32>(p, T_tokens, stream); \
-                   return go<T, 4, 2, 16>(p, T_tokens, stream); } while (0)
+#define GO(T) do { if (dk <= 64 && dv <= 128) return go<T, 1, 1, 32, false>(p, T_tokens, stream); \
+                   if (dk == 128 && dv == 128) return go<T, 2, 1, 32, true>(p, T_tokens, stream); \
+                   if (dk <= 128 && dv <= 128) return go<T, 2, 1, 32, false>(p, T_tokens, stream); \
+                   if (dk == 256 && dv == 256) return go<T, 4, 2, 16, true>(p, T_tokens, stream); \
+                   return go<T, 4, 2, 16, false>(p, T_tokens, stream); } while (0)
     if (dtype == QS_F32) GO(float);
     GO(__nv_bfloat16);
 #undef GO
