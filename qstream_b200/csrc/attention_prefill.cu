@@ -20,6 +20,11 @@
 // A row's result depends on its own sequence only: keys are visited page by page in position order
 // whatever else is in the batch and wherever the pages lie.
 //
+// NARROW: the cache holds 8-bit codes and a scale for each page and key head, a power of two, so that code * scale is a bfloat16 number
+// exactly (kv8.cu).  Four more warps take the place of the copies of keys and values: they read a page's codes, and write the numbers to
+// shared memory in the layout that the copies leave; everything behind is the same.  A page that was given a number that is not finite (its
+// scale is NaN) has keys of NaN and values of zero: a row that sees it gets NaN, weights of zero of the others times it stay zero.
+//
 // Sizes: head size a multiple of 16 up to 256 (tiles are padded to 64 columns with TMA's zero fill);
 // any number of heads and groups; pages of 64 tokens.
 #include "common.cuh"
@@ -36,10 +41,21 @@ constexpr int BM = 128;          // query rows per CTA = TMEM lanes
 constexpr int BN = 64;           // keys per block = one cache page
 constexpr int KC = 64;           // columns of one swizzled tile (128 bytes of bfloat16)
 constexpr int THREADS = 320;      // producer warp, MMA warp, eight softmax warps
+constexpr int DECODERS = 4;       // NARROW: warps that turn codes into numbers
 constexpr float RESCALE_THRESHOLD = 8.0f;        // log2 units
 
 struct TileInfo { int row_start, n_rows, qpos0, slot; };
 struct MaskOpts { int chunk, keep_first, maps, out_f32, head_gate; const float* sink; };
+struct Codes { const int8_t *k, *v; const float *k_scale, *v_scale; int n_slots, n_pages, rows; };
+
+// Two codes (bytes 2 i, 2 i + 1 of a word whose sign bits are flipped) times a scale, as bfloat16 numbers: 2^23 beside a byte is 2^23 + 128 + code, and
+// the multiply-add exact.
+__device__ __forceinline__ uint32_t two_numbers(uint32_t flipped, int i, float scale, float offset) {
+    const float a = fmaf(__uint_as_float(__byte_perm(flipped, 0x4b000000u, i ? 0x7442 : 0x7440)), scale, offset);
+    const float b = fmaf(__uint_as_float(__byte_perm(flipped, 0x4b000000u, i ? 0x7443 : 0x7441)), scale, offset);
+    const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
 
 // 2^x on the special-function unit (relative error about 2^-22; -inf gives 0).
 __device__ __forceinline__ float fast_exp2(float x) {
@@ -63,14 +79,14 @@ template <int NKC> constexpr int smem_bytes() {
     return q_bytes<NKC>() + 2 * kv_stages<NKC>() * kv_tile_bytes<NKC>() + 2 * P_BYTES + 1024 + 512 + 4 * BM * 2;
 }
 
-template <int NKC>
-__global__ void __launch_bounds__(THREADS, 1)
+template <int NKC, bool NARROW>
+__global__ void __launch_bounds__(THREADS + NARROW * DECODERS * 32, 1)
 attention_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                          const __grid_constant__ CUtensorMap map_v, __nv_bfloat16* __restrict__ out, size_t ldo,
                          const TileInfo* __restrict__ tiles, const int32_t* __restrict__ page_table, int max_pages,
                          int n_heads, int n_kv_heads, int dh, float scale_log2, int window,
                          int32_t* __restrict__ status, int dv, float cap_log2, float cap_k2,
-                         const __nv_bfloat16* __restrict__ gate, size_t ldg, const MaskOpts mask) {
+                         const __nv_bfloat16* __restrict__ gate, size_t ldg, const MaskOpts mask, const Codes codes) {
     // mask.chunk c > 0: a query sees the keys of its own chunk of c positions (counted from 0) instead of a window.
     // mask.keep_first n > 0 (with a window): the sequence's first n keys stay visible; their blocks are walked first.
     // mask.sink (may be null): exp(sink[head]) joins the row's sum, without a key or a value.  mask.maps m > 1: a key
@@ -110,6 +126,11 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     // work, so the last ones to start are the shortest (a causal tile's work grows with its position)
     const TileInfo tile = tiles[blockIdx.y];
     if (tile.n_rows <= 0) return;             // an unused entry of a tile list of fixed length (captured steps): the whole CTA leaves
+    if (NARROW && (tile.n_rows > BM || tile.slot < 0 || tile.slot >= codes.n_slots || tile.qpos0 < 0 || (tile.qpos0 + tile.n_rows - 1) / BN >= max_pages ||
+                   tile.row_start < 0 || tile.row_start + tile.n_rows > codes.rows)) {       // report, touch nothing
+        if (threadIdx.x == 0 && blockIdx.x == 0) atomicExch(status, 1);
+        return;
+    }
     const int head = blockIdx.x;
     const int maps = mask.maps > 1 ? mask.maps : 1;
     const int kvh = (head / maps) / ((n_heads / maps) / n_kv_heads);
@@ -124,7 +145,7 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
-        for (int s = 0; s < STAGES; ++s) { mbar_init(&k_full[s], 1); mbar_init(&v_full[s], 1); mbar_init(&k_empty[s], 1); mbar_init(&v_empty[s], 1); }
+        for (int s = 0; s < STAGES; ++s) { mbar_init(&k_full[s], NARROW ? DECODERS * 32 : 1); mbar_init(&v_full[s], NARROW ? DECODERS * 32 : 1); mbar_init(&k_empty[s], 1); mbar_init(&v_empty[s], 1); }
         mbar_init(&s_full[0], 1);
         mbar_init(&s_full[1], 1);
         mbar_init(&p_full[0], 2 * BM);
@@ -136,8 +157,10 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         *aborted = 0;
         mbar_fence_init();
         prefetch_tensormap(&map_q);
-        prefetch_tensormap(&map_k);
-        prefetch_tensormap(&map_v);
+        if (!NARROW) {
+            prefetch_tensormap(&map_k);
+            prefetch_tensormap(&map_v);
+        }
     }
     if (warp == 1) { tmem_alloc(tmem_slot, TMEM_COLS); tmem_relinquish(); }
     tc_fence_before_sync();
@@ -153,6 +176,7 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 #pragma unroll
             for (int c = 0; c < NKC; ++c)
                 if (c < n_kc) tma_load_2d(q_smem + c * BM * KC * 2, &map_q, q_full, head * dh + c * KC, tile.row_start);
+            if constexpr (!NARROW) {
             const int32_t* pages = page_table + (size_t)tile.slot * max_pages;
             auto tile_row = [&](int j) {
                 int page = pages[block_of(j)];
@@ -188,6 +212,65 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 if (j + 1 < n_blocks) ok = load_k(j + 1);
                 if (ok) ok = load_v(j);
             }
+            }
+        }
+    } else if (NARROW && warp >= THREADS / 32) {
+        // ------------------------------------------------------------------ codes to numbers
+        // A thread takes pieces of 16 codes of a row: 32 bytes, two chunks of the swizzled row of 64 numbers.  The codes of the next block are
+        // on their way while a block's place is waited for.
+        const int me = threadIdx.x - THREADS;
+        const int32_t* pages = page_table + (size_t)tile.slot * max_pages;
+        constexpr int PIECES = BN * NKC * KC / 16 / (DECODERS * 32);     // of a thread, keys or values each: 2 NKC
+        auto page_of = [&](int j) {
+            const int page = pages[block_of(j)];
+            if (page < 0 || page >= codes.n_pages) { if (me == 0) atomicExch(status, 3); return 0; }       // still fill the stage so nobody waits for it
+            return page;
+        };
+        auto load = [&](uint4 (&raw)[PIECES], const int8_t* src, int d) {       // rows of d codes; pieces across a row, then down
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                const int e = i * DECODERS * 32 + me, row = e / (NKC * 4), c = e % (NKC * 4);
+                raw[i] = c * 16 < d ? __ldg(reinterpret_cast<const uint4*>(src + (size_t)row * d + c * 16)) : make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+            }
+        };
+        auto store = [&](const uint4 (&raw)[PIECES], uint8_t* dst, int d, float scale) {
+            const float offset = -8388736.f * scale;
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                const int e = i * DECODERS * 32 + me, row = e / (NKC * 4), c = e % (NKC * 4);
+                const bool in = c * 16 < d;               // beyond the row: zeros, as the copies fill them in
+                const uint32_t w[4] = {raw[i].x ^ 0x80808080u, raw[i].y ^ 0x80808080u, raw[i].z ^ 0x80808080u, raw[i].w ^ 0x80808080u};
+                uint8_t* tile_at = dst + (c >> 2) * BN * KC * 2 + row * 128;
+                uint32_t o[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) o[k] = in ? two_numbers(w[k >> 1], k & 1, scale, offset) : 0u;
+                *reinterpret_cast<uint4*>(tile_at + ((((c & 3) * 2) ^ (row & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+                *reinterpret_cast<uint4*>(tile_at + ((((c & 3) * 2 + 1) ^ (row & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+            }
+        };
+        uint4 kr[PIECES], vr[PIECES];
+        float ks, vs;
+        auto fetch = [&](int j) {
+            const size_t at = (size_t)page_of(j) * n_kv_heads + kvh;
+            ks = codes.k_scale[at];
+            vs = codes.v_scale[at];
+            load(kr, codes.k + at * BN * dh, dh);
+            load(vr, codes.v + at * BN * dv, dv);
+        };
+        fetch(0);
+        for (int j = 0; j < n_blocks; ++j) {
+            const int st = j % STAGES;
+            uint8_t* k_tile = kv_smem + (size_t)st * 2 * KV_TILE;
+            if (!mbar_wait(&k_empty[st], ((j / STAGES) & 1) ^ 1)) { atomicExch(status, 111); *aborted = 1; break; }
+            const bool nan = isnan(ks) || isnan(vs);
+            store(kr, k_tile, dh, nan ? __uint_as_float(0x7fffffffu) : ks);
+            fence_proxy_async_smem();
+            mbar_arrive(&k_full[st]);
+            if (!mbar_wait(&v_empty[st], ((j / STAGES) & 1) ^ 1)) { atomicExch(status, 110); *aborted = 1; break; }
+            store(vr, k_tile + KV_TILE, dv, nan ? 0.f : vs);
+            fence_proxy_async_smem();
+            mbar_arrive(&v_full[st]);
+            if (j + 1 < n_blocks) fetch(j + 1);
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------------ MMA issuer
@@ -329,7 +412,8 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             // swizzled K-major layout; the row sum is taken in 32-bit over two independent chains.
             if (ok) {
                 uint8_t* prow = p_smem + (j & 1) * P_BYTES + (size_t)r * 128;
-                const float neg_m = m == -INFINITY ? -INFINITY : -m;          // a row with no visible key so far: all weights 0
+                // a row with no visible key so far: all weights 0 (NARROW: 2^-inf, and NaN where what it sees is NaN)
+                const float neg_m = m == -INFINITY ? (NARROW ? 0.f : -INFINITY) : -m;
                 float ps0 = 0.f, ps1 = 0.f;
 #pragma unroll
                 for (int ch = 0; ch < 4; ++ch) {
@@ -362,10 +446,10 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         float l_all = lsum[r] + lsum[BM + r];
         // the sink: one more term of the softmax's sum, in the units of the row's maximum (log2, scaled); both of the
         // row's threads hold the same m
-        if (mask.sink && m != -INFINITY) l_all += exp2f(mask.sink[head] * 1.4426950408889634f - m);
+        if (mask.sink && (NARROW || m != -INFINITY)) l_all += exp2f(mask.sink[head] * 1.4426950408889634f - m);
         if (ok && !*aborted) {
             tc_fence_after_sync();
-            float inv = l_all > 0.f ? 1.0f / l_all : 0.f;
+            float inv = (NARROW ? l_all != 0.f : l_all > 0.f) ? 1.0f / l_all : 0.f;
             if (gate && mask.head_gate && valid) inv *= sigmoid_f32(__bfloat162float(gate[(size_t)(tile.row_start + r) * ldg + head]));
             __nv_bfloat16* orow = out + (size_t)(tile.row_start + r) * ldo + (size_t)head * dv;
             float* orow32 = reinterpret_cast<float*>(out) + (size_t)(tile.row_start + r) * ldo + (size_t)head * dv;
@@ -452,22 +536,22 @@ int make_map(CUtensorMap* out, const void* ptr, long long rows, long long cols, 
     return QS_OK;
 }
 
-template <int NKC>
+template <int NKC, bool NARROW>
 int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, void* out, long long ldo,
            const TileInfo* tiles, int n_tiles, const int32_t* page_table, int max_pages, int n_heads, int n_kv_heads,
            int dh, float scale_log2, int window, int32_t* status, int dv, float cap_log2, float cap_k2, const void* gate,
-           long long ldg, const MaskOpts& mask, cudaStream_t stream) {
+           long long ldg, const MaskOpts& mask, const Codes& codes, cudaStream_t stream) {
     static bool configured = false;
     if (!configured) {
-        cudaError_t e = cudaFuncSetAttribute(attention_prefill_kernel<NKC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        cudaError_t e = cudaFuncSetAttribute(attention_prefill_kernel<NKC, NARROW>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              smem_bytes<NKC>());
         if (e != cudaSuccess) return qs_fail(QS_ERR_INTERNAL, "attention_prefill: shared memory of %d bytes refused: %s",
                                              smem_bytes<NKC>(), cudaGetErrorString(e));
         configured = true;
     }
-    attention_prefill_kernel<NKC><<<dim3(n_heads, n_tiles), THREADS, smem_bytes<NKC>(), stream>>>(
+    attention_prefill_kernel<NKC, NARROW><<<dim3(n_heads, n_tiles), THREADS + NARROW * DECODERS * 32, smem_bytes<NKC>(), stream>>>(
         mq, mk, mv, (__nv_bfloat16*)out, (size_t)ldo, tiles, page_table, max_pages, n_heads, n_kv_heads, dh,
-        scale_log2, window, status, dv, cap_log2, cap_k2, (const __nv_bfloat16*)gate, (size_t)ldg, mask);
+        scale_log2, window, status, dv, cap_log2, cap_k2, (const __nv_bfloat16*)gate, (size_t)ldg, mask, codes);
     return qs_check_launch("attention_prefill");
 }
 
@@ -523,8 +607,40 @@ QS_API int qs_attention_prefill_masked(void* out, long long ldo, const void* q, 
     const TileInfo* ti = reinterpret_cast<const TileInfo*>(tiles);
     const MaskOpts mask = {chunk, keep_first, maps, out_f32, head_gate, sink};
     const int nkc = ((dh > dv ? dh : dv) + KC - 1) / KC;
-#define GO(NKC) return launch<NKC>(mq, mk, mv, out, ldo, ti, n_tiles, page_table, max_pages, n_heads, n_kv_heads, dh, \
-                                   scale_log2, window, status, dv, cap_log2, cap_k2, gate, ldg, mask, stream)
+#define GO(NKC) return launch<NKC, false>(mq, mk, mv, out, ldo, ti, n_tiles, page_table, max_pages, n_heads, n_kv_heads, dh, \
+                                          scale_log2, window, status, dv, cap_log2, cap_k2, gate, ldg, mask, Codes(), stream)
+    if (nkc == 1) GO(1);
+    if (nkc == 2) GO(2);
+    if (nkc == 3) GO(3);
+    GO(4);
+#undef GO
+}
+
+// The same over 8-bit pages (layout: kv8.cu): out [T, n_heads * dv] bfloat16 or float32 (out_f32).  Status 1: a tile outside the rows, the
+// slots or the page table (nothing is written for it), 3: a page that its sequence does not hold.
+QS_API int qs_kv8_prefill(void* out, int out_f32, long long ldo, const void* q, long long ldq, int T_tokens, const int8_t* k_cache, const int8_t* v_cache,
+                          const float* k_scale, const float* v_scale, int n_pages, const int32_t* page_table, int n_slots, int max_pages, const int32_t* tiles,
+                          int n_tiles, int n_heads, int n_kv_heads, int dh, int dv, float scale, int window, int chunk, int keep_first, const float* sink,
+                          float softcap, int32_t* status, cudaStream_t stream) {
+    if (n_tiles == 0 || T_tokens == 0) return QS_OK;
+    QS_REQUIRE(T_tokens > 0 && n_tiles > 0 && n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0 && n_pages > 0 && n_slots > 0 && max_pages > 0, "kv8 prefill: bad sizes");
+    QS_REQUIRE(chunk >= 0 && keep_first >= 0 && window >= 0 && !(chunk > 0 && window > 0), "kv8 prefill: a window of %d and chunks of %d", window, chunk);
+    QS_REQUIRE(dh % 16 == 0 && dh >= 16 && dh <= 256 && dv % 16 == 0 && dv >= 16 && dv <= 256, "kv8 prefill: head sizes %d and %d (multiples of 16 up to 256)", dh, dv);
+    QS_REQUIRE(scale > 0.f && softcap >= 0.f, "kv8 prefill: the scale must be positive and the cap not negative");
+    QS_REQUIRE(ldq % 8 == 0 && ldo % (out_f32 ? 4 : 8) == 0 && ((uintptr_t)q % 16) == 0 && ((uintptr_t)out % 16) == 0 && ((uintptr_t)k_cache % 16) == 0 &&
+               ((uintptr_t)v_cache % 16) == 0, "kv8 prefill: rows and pages must be 16-byte aligned");
+    QS_REQUIRE(n_tiles <= 65535 && n_heads <= 65535, "kv8 prefill: %d tiles of queries are too many for the grid", n_tiles);
+    CUtensorMap mq;
+    const int rc = make_map(&mq, q, T_tokens, (long long)n_heads * dh, ldq, BM);
+    if (rc != QS_OK) return rc;
+    const float log2e = 1.4426950408889634f;
+    const float scale_log2 = scale * log2e, cap_log2 = softcap > 0.f ? softcap * log2e : 0.f, cap_k2 = softcap > 0.f ? 2.0f * log2e * scale / softcap : 0.f;
+    const TileInfo* ti = reinterpret_cast<const TileInfo*>(tiles);
+    const MaskOpts mask = {chunk, keep_first, 1, out_f32, 0, sink};
+    const Codes codes = {k_cache, v_cache, k_scale, v_scale, n_slots, n_pages, T_tokens};
+    const int nkc = ((dh > dv ? dh : dv) + KC - 1) / KC;
+#define GO(NKC) return launch<NKC, true>(mq, mq, mq, out, ldo, ti, n_tiles, page_table, max_pages, n_heads, n_kv_heads, dh, \
+                                         scale_log2, window, status, dv, cap_log2, cap_k2, nullptr, 0, mask, codes, stream)
     if (nkc == 1) GO(1);
     if (nkc == 2) GO(2);
     if (nkc == 3) GO(3);

@@ -171,7 +171,10 @@ kv8_attention_kernel(TO* __restrict__ out, const T* __restrict__ q, const Attend
         const int i = blockIdx.y & 127;
         if (i >= t[1]) return;
         row = t[0] + i; pos = t[2] + i; slot = t[3];
-        if (row < 0 || row >= p.T) return;
+        if (t[1] > 128 || t[0] < 0 || t[0] + t[1] > p.T || slot < 0 || slot >= p.n_slots || t[2] < 0 || (t[2] + t[1] - 1) >> 6 >= p.max_pages) {      // the whole tile: report, write nothing
+            if (lane == 0) atomicExch(p.status, 1);
+            return;
+        }
     } else {
         row = blockIdx.y; slot = p.tok_slot[row]; pos = p.tok_pos[row];
     }

@@ -18,11 +18,11 @@ from .q4 import TYPES, _on_current_device, _refuse
 PAGE_TOKENS = 64
 MAX_SPLIT_CONTEXT = 4096 * 128      # what the merge of the keys' parts holds for any head size; longer contexts go a row at a time
 
-_store = _read = _attention = _decode = _scratch = None
+_store = _read = _attention = _decode = _scratch = _prefill = None
 
 
 def _bind():
-    global _store, _read, _attention, _decode, _scratch
+    global _store, _read, _attention, _decode, _scratch, _prefill
     if _store is None:
         _read = ops.bind("qs_kv8_read_pages", [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p])
         _attention = ops.bind("qs_kv8_attention", [
@@ -32,6 +32,9 @@ def _bind():
             c_void_p, c_int, c_longlong, c_void_p, c_int, c_longlong, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
             c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p, c_float, c_int, c_void_p, c_void_p, c_void_p])
         _scratch = ops.bind("qs_kv8_decode_scratch", [c_int, c_int, c_int, c_int, c_int], c_longlong)
+        _prefill = ops.bind("qs_kv8_prefill", [
+            c_void_p, c_int, c_longlong, c_void_p, c_longlong, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p,
+            c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p, c_float, c_void_p, c_void_p])
         _store = ops.bind("qs_kv8_store", [
             c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong, c_float, c_int,
             c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
@@ -208,6 +211,14 @@ def prefill(q, n_heads, n_kv_heads, head_dim, scale, window, tiles, page_table, 
     _bind()
     if padded:
         out.zero_()
+    wide = int(out.dtype == torch.float32)
+    if (q.dtype == torch.bfloat16 and head_dim % 16 == 0 and dv % 16 == 0 and head_dim <= 256 and dv <= 256 and scale > 0 and tiles.shape[0] <= 65535
+            and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0 and out.stride(0) % (4 if wide else 8) == 0 and out.data_ptr() % 16 == 0):
+        ops.check(_prefill(ops.ptr(out), wide, out.stride(0), ops.ptr(q), q.stride(0), T, ops.ptr(k_cache), ops.ptr(v_cache), ops.ptr(k_scale), ops.ptr(v_scale),
+                           k_cache.shape[0], ops.ptr(page_table), page_table.shape[0], page_table.shape[1], ops.ptr(tiles), tiles.shape[0], n_heads, n_kv_heads,
+                           head_dim, dv, float(scale), int(window), int(chunk), int(keep_first), ops.ptr(sink), float(softcap or 0.0), ops.ptr(status),
+                           ops.stream()))
+        return out
     for a in range(0, tiles.shape[0], 511):
         b = min(tiles.shape[0], a + 511)
         ops.check(_attention(ops.ptr(out), ops.dtype_code(out), out.stride(0), ops.ptr(q), ops.dtype_code(q), q.stride(0), T, None, None, ops.ptr(tiles[a:b]), b - a,

@@ -309,6 +309,25 @@ def test_rows_that_cannot_be_read_are_reported():
             assert (got[1] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_tiles_that_cannot_be_read_are_reported(dtype):
+    rng = np.random.default_rng(17)
+    pages = U.paged(rng, [200, 70], 1, 64, 64)
+    dev, table = device(pages)
+    q = torch.tensor(rng.normal(size=(20, 64))).to(TYPES[dtype]).cuda()
+    good = (0, 10, 190, 0)
+    for bad, code in (((10, 11, 0, 1), 1), ((-1, 5, 0, 1), 1), ((10, 5, 0, 2), 1), ((10, 5, 0, -1), 1), ((10, 5, -3, 1), 1), ((10, 5, 254, 0), 1), ((10, 5, 130, 1), 3)):
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        out = torch.full((20, 64), 7.0, dtype=TYPES[dtype], device="cuda")
+        kv8.prefill(q, 1, 1, 64, 0.125, 0, i32([good, bad]), table, 64, *dev, status, out=out)
+        assert int(status.item()) == code, bad
+        want, bound = U.attention(U.f64(q).reshape(20, 1, 64), pages[:2], pages[2:4], [0] * 10 + [-1] * 10, list(range(190, 200)) + [0] * 10, pages[4], 1, 0.125,
+                                  wide_weights=dtype == "f32", out_bf16=dtype == "bf16")
+        check(out[:10], want[:10], bound[:10] + (2.0 ** -8 * 127 * float(pages[3].max()) if dtype == "bf16" else 0))
+        if code == 1:
+            assert (out[10:] == 7).all()
+
+
 def test_a_row_does_not_depend_on_its_batch():
     rng = np.random.default_rng(13)
     lens = [1000, 3, 517, 64, 2000, 129]
