@@ -54,12 +54,82 @@ struct StoreArgs {
     float lam;
 };
 
+__device__ __forceinline__ void store16(float* dst, const float (&x)[16]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(dst)[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+}
+__device__ __forceinline__ void store16(__nv_bfloat16* dst, const float (&x)[16]) {
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const __nv_bfloat162 r = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&r);
+    }
+    reinterpret_cast<uint4*>(dst)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    reinterpret_cast<uint4*>(dst)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+}
+
+// 16 elements of a row from d on; those of a row's first R dims rotated (`cs`: the row's angles).
+template <typename T>
+__device__ __forceinline__ void load16(const T* __restrict__ row, float (&x)[16]) {
+    float a[8], b[8];
+    load8_as_f32(row, sizeof(T) == 4 ? QS_F32 : QS_BF16, 0, a);
+    load8_as_f32(row, sizeof(T) == 4 ? QS_F32 : QS_BF16, 8, b);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { x[i] = a[i]; x[8 + i] = b[i]; }
+}
+template <typename T>
+__device__ __forceinline__ void rotated16(const T* __restrict__ row, int d, const float* __restrict__ cs, int R, int half_layout, float (&x)[16]) {
+    load16(row + d, x);
+    if (d >= R) return;
+    const int rp = R >> 1;
+    if (half_layout) {
+        const bool second = d >= rp;
+        float y[16];
+        load16(row + (second ? d - rp : d + rp), y);
+        const float4* angle = reinterpret_cast<const float4*>(cs + 2 * (second ? d - rp : d));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float4 c = angle[i];
+            x[2 * i] = second ? __fadd_rn(__fmul_rn(y[2 * i], c.y), __fmul_rn(x[2 * i], c.x)) : __fsub_rn(__fmul_rn(x[2 * i], c.x), __fmul_rn(y[2 * i], c.y));
+            x[2 * i + 1] = second ? __fadd_rn(__fmul_rn(y[2 * i + 1], c.w), __fmul_rn(x[2 * i + 1], c.z)) : __fsub_rn(__fmul_rn(x[2 * i + 1], c.z), __fmul_rn(y[2 * i + 1], c.w));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float4 c = reinterpret_cast<const float4*>(cs + d)[i];
+            const float a0 = x[4 * i], b0 = x[4 * i + 1], a1 = x[4 * i + 2], b1 = x[4 * i + 3];
+            x[4 * i] = __fsub_rn(__fmul_rn(a0, c.x), __fmul_rn(b0, c.y));
+            x[4 * i + 1] = __fadd_rn(__fmul_rn(a0, c.y), __fmul_rn(b0, c.x));
+            x[4 * i + 2] = __fsub_rn(__fmul_rn(a1, c.z), __fmul_rn(b1, c.w));
+            x[4 * i + 3] = __fadd_rn(__fmul_rn(a1, c.w), __fmul_rn(b1, c.z));
+        }
+    }
+}
+
+// Four numbers, already divided by the scale, as a word of codes.
+__device__ __forceinline__ uint32_t four_codes(float a, float b, float c, float d) {
+    const float v[4] = {a, b, c, d};
+    uint32_t r = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r |= (uint32_t)(max(-127, min(127, __float2int_rn(v[i]))) & 255) << (8 * i);
+    return r;
+}
+
 // n rows of one page and head, from row `a` of the page on: the scale that holds them and what is there already, then the codes.
-// value(i, d): element d of new row i.
-template <typename F>
+// VEC: value(i, d, x) gives elements d .. d + 15 of new row i, else element d.  The rows are read twice, the second time from the caches: they are too
+// many for the registers of a block, and the rotation is cheap.
+template <bool VEC, typename F>
 __device__ __forceinline__ void store_run(int8_t* __restrict__ codes, float* __restrict__ scale, int a, int n, int dim, uint32_t* scratch, F value) {
+    constexpr int E = VEC ? 16 : 1;
+    const int pieces = dim / E, items = n * pieces;
     uint32_t most = 0;                                   // as bits: numbers that are not finite are above all others
-    for (int e = threadIdx.x; e < n * dim; e += blockDim.x) most = max(most, __float_as_uint(value(e / dim, e % dim)) & 0x7fffffffu);
+    for (int e = threadIdx.x; e < items; e += blockDim.x) {
+        float x[E];
+        value(e / pieces, e % pieces * E, x);
+#pragma unroll
+        for (int i = 0; i < E; ++i) most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
+    }
     most = block_max(most, scratch);
     const float before = a > 0 ? *scale : 0.f;
     const float need = most >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : most == 0 ? 0.f : scale_for(most);
@@ -68,82 +138,174 @@ __device__ __forceinline__ void store_run(int8_t* __restrict__ codes, float* __r
     if (threadIdx.x == 0) *scale = after;
     if (a > 0 && after != before && !isnan(after)) {
         const float shrink = before / after;
-        for (int e = threadIdx.x; e < a * dim; e += blockDim.x) codes[e] = (int8_t)__float2int_rn((float)codes[e] * shrink);
+        if (VEC) {
+            uint32_t* words = reinterpret_cast<uint32_t*>(codes);
+            for (int e = threadIdx.x; e < a * dim / 4; e += blockDim.x) {
+                const uint32_t w = words[e];
+                words[e] = four_codes((float)(int8_t)w * shrink, (float)(int8_t)(w >> 8) * shrink, (float)(int8_t)(w >> 16) * shrink, (float)(int8_t)(w >> 24) * shrink);
+            }
+        } else {
+            for (int e = threadIdx.x; e < a * dim; e += blockDim.x) codes[e] = (int8_t)__float2int_rn((float)codes[e] * shrink);
+        }
     }
     const float inv = after > 0.f ? 1.0f / after : 0.f;  // NaN: the codes say nothing, and 0
-    for (int e = threadIdx.x; e < n * dim; e += blockDim.x)
-        codes[(size_t)a * dim + e] = (int8_t)(inv > 0.f ? max(-127, min(127, __float2int_rn(value(e / dim, e % dim) * inv))) : 0);
+    for (int e = threadIdx.x; e < items; e += blockDim.x) {
+        float x[E];
+        value(e / pieces, e % pieces * E, x);
+#pragma unroll
+        for (int i = 0; i < E; ++i) x[i] = inv > 0.f ? x[i] * inv : 0.f;
+        if (VEC) {
+            constexpr int S = VEC ? 4 : 0;
+            *reinterpret_cast<uint4*>(codes + (size_t)a * dim + e * 16) =
+                make_uint4(four_codes(x[0], x[S / 4], x[S / 2], x[3 * S / 4]), four_codes(x[S], x[5 * S / 4], x[6 * S / 4], x[7 * S / 4]),
+                           four_codes(x[2 * S], x[9 * S / 4], x[10 * S / 4], x[11 * S / 4]), four_codes(x[3 * S], x[13 * S / 4], x[14 * S / 4], x[15 * S / 4]));
+        } else {
+            codes[(size_t)a * dim + e] = (int8_t)max(-127, min(127, __float2int_rn(x[0])));
+        }
+    }
 }
 
-// blockIdx.x: `rows` consecutive rows of the step; blockIdx.y: a key head, then blocks that rotate the queries of these rows.
+// blockIdx.x: `rows` (up to 32) consecutive rows of the step; blockIdx.y: a key head, then blocks that rotate the queries of these rows.
 // A run is the rows of one sequence that fall into one page: consecutive rows of ascending positions.  The block of a run's first row takes
 // the whole run, so that a page's scale has one writer; a second run for the same page in one call is reported (status 5) and not written.
-template <typename T>
-__global__ void __launch_bounds__(128)
-kv8_store_kernel(T* __restrict__ q_out, const T* q, const T* __restrict__ k, const T* __restrict__ v, const T* __restrict__ v_first, const StoreArgs p) {
+// VEC: rows, angles and pages in pieces of 16 elements, on their boundaries.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256)
+kv8_store_kernel(T* q_out, const T* q, const T* __restrict__ k, const T* __restrict__ v, const T* __restrict__ v_first, const StoreArgs p) {
+    constexpr int E = VEC ? 16 : 1;
     __shared__ uint32_t scratch[33];
-    const int row0 = blockIdx.x * p.rows, rows = min(p.rows, p.T - row0);
+    grid_dep_launch();
+    grid_dep_wait();
+    const int row0 = blockIdx.x * p.rows, rows = min(p.rows, p.T - row0), lane = threadIdx.x & 31;
     const bool rotate = p.cos_sin != nullptr && p.R > 0;
     if ((int)blockIdx.y >= p.n_kv_heads) {
-        const int half = p.dk >> 1, rp = rotate ? p.R >> 1 : 0, items = rows * p.n_heads * half;
+        // an item: 16 (VEC) or 1 pairs that turn, or as many plain elements of both halves of the rest
+        const int rp = rotate ? p.R >> 1 : 0, turning = VEC && !p.half_layout ? rp / 8 : rp / E, plain = q_out == q ? 0 : (p.dk - 2 * rp) / E;
+        const int per_head = turning + plain, per_row = p.n_heads * per_head, items = rows * per_row;
         for (int e = (blockIdx.y - p.n_kv_heads) * blockDim.x + threadIdx.x; e < items; e += p.q_blocks * blockDim.x) {
-            const int i = e / (p.n_heads * half), r = row0 + i, head = (e - i * p.n_heads * half) / half, j = e % half;
+            const int i = e / per_row, r = row0 + i, rest = e - i * per_row, head = rest / per_head, j = rest - head * per_head;
             const int slot = p.tok_slot[r], pos = p.tok_pos[r];
             const bool fits = slot >= 0 && pos >= 0 && pos < p.max_pos;
             if (rotate && slot >= 0 && !fits && head == 0 && j == 0) atomicExch(p.status, 1);
             const T* src = q + (size_t)r * p.ldq + (size_t)head * p.dk;
             T* dst = q_out + (size_t)r * p.ldqo + (size_t)head * p.dk;
-            if (j < rp && fits) {
-                const float c = p.cos_sin[(size_t)pos * p.R + 2 * j], s = p.cos_sin[(size_t)pos * p.R + 2 * j + 1];
+            if (!fits && dst == src) continue;
+            const float* cs = p.cos_sin + (size_t)pos * p.R;
+            if constexpr (VEC) {
+                auto copy = [&](int d) {
+                    float x[16];
+                    load16(src + d, x);
+                    store16(dst + d, x);
+                };
+                if (j >= turning) copy(2 * rp + (j - turning) * 16);
+                else if (p.half_layout) {
+                    if (!fits) { copy(j * 16); copy(j * 16 + rp); continue; }
+                    float x[16], y[16];
+                    load16(src + j * 16, x);
+                    load16(src + j * 16 + rp, y);
+#pragma unroll
+                    for (int u = 0; u < 16; ++u) {
+                        const float c = cs[2 * (j * 16 + u)], s = cs[2 * (j * 16 + u) + 1], a = x[u], b = y[u];
+                        x[u] = a * c - b * s;
+                        y[u] = a * s + b * c;
+                    }
+                    store16(dst + j * 16, x);
+                    store16(dst + j * 16 + rp, y);
+                } else {
+                    if (!fits) { copy(j * 16); continue; }
+                    float x[16];
+                    load16(src + j * 16, x);
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) {
+                        const float c = cs[j * 16 + 2 * u], s = cs[j * 16 + 2 * u + 1], a = x[2 * u], b = x[2 * u + 1];
+                        x[2 * u] = a * c - b * s;
+                        x[2 * u + 1] = a * s + b * c;
+                    }
+                    store16(dst + j * 16, x);
+                }
+            } else if (j < turning) {
                 const int ia = p.half_layout ? j : 2 * j, ib = p.half_layout ? j + rp : 2 * j + 1;
                 const float a = to_f32(src[ia]), b = to_f32(src[ib]);
-                dst[ia] = from_f32<T>(a * c - b * s);
-                dst[ib] = from_f32<T>(a * s + b * c);
-            } else if (dst != src) {
-                const int ia = p.half_layout && j < rp ? j : 2 * j, ib = p.half_layout && j < rp ? j + rp : 2 * j + 1;
-                dst[ia] = src[ia];
-                dst[ib] = src[ib];
+                const float c = fits ? cs[2 * j] : 1.f, s = fits ? cs[2 * j + 1] : 0.f;
+                dst[ia] = fits ? from_f32<T>(a * c - b * s) : src[ia];
+                dst[ib] = fits ? from_f32<T>(a * s + b * c) : src[ib];
+            } else {
+                dst[2 * rp + j - turning] = src[2 * rp + j - turning];
             }
         }
         return;
     }
     const int kvh = blockIdx.y;
-    for (int r = row0; r < row0 + rows; ++r) {
-        const int slot = p.tok_slot[r], pos = p.tok_pos[r];
-        if (slot < 0) continue;
+    // which of the rows begin a run
+    bool begins = false;
+    if (lane < rows) {
+        const int r = row0 + lane, slot = p.tok_slot[r], pos = p.tok_pos[r];
         const bool bad = slot >= p.n_slots || pos < 0 || (pos >> 6) >= p.max_pages || (rotate && pos >= p.max_pos);
-        if (bad) { if (threadIdx.x == 0 && kvh == 0) atomicExch(p.status, 1); continue; }
-        if (r > 0 && p.tok_slot[r - 1] == slot && p.tok_pos[r - 1] == pos - 1 && (pos & (PAGE - 1)) != 0) continue;       // inside a run
+        if (slot >= 0 && bad && threadIdx.x < 32 && kvh == 0) atomicExch(p.status, 1);
+        begins = slot >= 0 && !bad && !(r > 0 && (pos & (PAGE - 1)) != 0 && p.tok_slot[r - 1] == slot && p.tok_pos[r - 1] == pos - 1);
+    }
+    for (uint32_t todo = __ballot_sync(0xffffffffu, begins); todo != 0; todo &= todo - 1) {
+        const int r = row0 + __ffs(todo) - 1, slot = p.tok_slot[r], pos = p.tok_pos[r];
         const int page = p.page_table[(size_t)slot * p.max_pages + (pos >> 6)];
         if (page < 0 || page >= p.n_pages) { if (threadIdx.x == 0) atomicExch(p.status, 2); continue; }
         int again = 0;
         for (int i = threadIdx.x; i < r; i += blockDim.x) again |= p.tok_slot[i] == slot && (p.tok_pos[i] >> 6) == (pos >> 6);
         const int a = pos & (PAGE - 1);
-        int n = 1;
-        while (a + n < PAGE && r + n < p.T && p.tok_slot[r + n] == slot && p.tok_pos[r + n] == pos + n && !(rotate && pos + n >= p.max_pos)) ++n;
+        // the run's length: the first row behind it, 64 rows looked at by two lanes' turns
+        int n = PAGE - a;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int i = u * 32 + lane;
+            const bool ends = i > 0 && i < PAGE - a && !(r + i < p.T && p.tok_slot[r + i] == slot && p.tok_pos[r + i] == pos + i && !(rotate && pos + i >= p.max_pos));
+            const uint32_t found = __ballot_sync(0xffffffffu, ends);
+            if (found) n = min(n, u * 32 + __ffs(found) - 1);
+        }
         if (__syncthreads_or(again)) { if (threadIdx.x == 0) atomicExch(p.status, 5); continue; }
         const size_t at = (size_t)page * p.n_kv_heads + kvh;
-        store_run(p.k_cache + at * PAGE * p.dk, p.k_scale + at, a, n, p.dk, scratch, [&](int i, int d) {
-            return rotated(k + (size_t)(r + i) * p.ldk + (size_t)kvh * p.dk, d, p.cos_sin + (size_t)(pos + i) * p.R, rotate ? p.R : 0, p.half_layout);
+        store_run<VEC>(p.k_cache + at * PAGE * p.dk, p.k_scale + at, a, n, p.dk, scratch, [&](int i, int d, float (&x)[E]) {
+            const T* row = k + (size_t)(r + i) * p.ldk + (size_t)kvh * p.dk;
+            const float* cs = p.cos_sin + (size_t)(pos + i) * p.R;
+            if constexpr (VEC) rotated16(row, d, cs, rotate ? p.R : 0, p.half_layout, x);
+            else x[0] = rotated(row, d, cs, rotate ? p.R : 0, p.half_layout);
         });
-        store_run(p.v_cache + at * PAGE * p.dv, p.v_scale + at, a, n, p.dv, scratch, [&](int i, int d) {
-            const float x = to_f32(v[(size_t)(r + i) * p.ldv + (size_t)kvh * p.dv + d]);
-            return v_first ? __fadd_rn(__fmul_rn(1.0f - p.lam, x), __fmul_rn(p.lam, to_f32(v_first[(size_t)(r + i) * p.ldvf + (size_t)kvh * p.dv + d]))) : x;
+        store_run<VEC>(p.v_cache + at * PAGE * p.dv, p.v_scale + at, a, n, p.dv, scratch, [&](int i, int d, float (&x)[E]) {
+            const T* row = v + (size_t)(r + i) * p.ldv + (size_t)kvh * p.dv + d;
+            if constexpr (VEC) load16(row, x);
+            else x[0] = to_f32(*row);
+            if (v_first) {
+                const T* first = v_first + (size_t)(r + i) * p.ldvf + (size_t)kvh * p.dv + d;
+#pragma unroll
+                for (int u = 0; u < E; ++u) x[u] = __fadd_rn(__fmul_rn(1.0f - p.lam, x[u]), __fmul_rn(p.lam, to_f32(first[u])));
+            }
         });
     }
 }
 
 // Pages as the numbers they stand for; a page that does not exist gives NaN.
-template <typename T>
-__global__ void kv8_read_pages_kernel(T* __restrict__ out, const int8_t* __restrict__ codes, const float* __restrict__ scales, const int32_t* __restrict__ pages,
-                                      int n_pages, int n_kv_heads, int dim) {
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256)
+kv8_read_pages_kernel(T* __restrict__ out, const int8_t* __restrict__ codes, const float* __restrict__ scales, const int32_t* __restrict__ pages,
+                      int n_pages, int n_kv_heads, int dim) {
+    grid_dep_launch();
+    grid_dep_wait();
     const int page = pages[blockIdx.y], kvh = blockIdx.x;
     const bool there = page >= 0 && page < n_pages;
     const size_t at = there ? (size_t)page * n_kv_heads + kvh : 0;
     const float scale = there ? scales[at] : __uint_as_float(0x7fffffffu);
     const int8_t* src = codes + at * PAGE * dim;
     T* dst = out + ((size_t)blockIdx.y * n_kv_heads + kvh) * PAGE * dim;
-    for (int e = threadIdx.x; e < PAGE * dim; e += blockDim.x) dst[e] = from_f32<T>((float)src[e] * scale);
+    if (VEC) {
+        for (int e = threadIdx.x; e < PAGE * dim / 16; e += blockDim.x) {
+            const uint4 raw = __ldg(reinterpret_cast<const uint4*>(src) + e);
+            const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+            float x[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = (float)(int8_t)(w[i >> 2] >> (8 * (i & 3))) * scale;
+            store16(dst + e * 16, x);
+        }
+    } else {
+        for (int e = threadIdx.x; e < PAGE * dim; e += blockDim.x) dst[e] = from_f32<T>((float)src[e] * scale);
+    }
 }
 
 // One warp per row and query head, for every size: 32 keys at a time in position order, a key to a lane; the running maximum and
@@ -241,9 +403,11 @@ kv8_attention_kernel(TO* __restrict__ out, const T* __restrict__ q, const Attend
 }
 
 template <typename T>
-int store_launch(void* q_out, const void* q, const void* k, const void* v, const void* v_first, const StoreArgs& p, cudaStream_t stream) {
-    kv8_store_kernel<T><<<dim3((p.T + p.rows - 1) / p.rows, p.n_kv_heads + p.q_blocks), 128, 0, stream>>>(
-        (T*)q_out, (const T*)q, (const T*)k, (const T*)v, (const T*)v_first, p);
+int store_launch(void* q_out, const void* q, const void* k, const void* v, const void* v_first, const StoreArgs& p, bool vec, cudaStream_t stream) {
+    const dim3 grid((p.T + p.rows - 1) / p.rows, p.n_kv_heads + p.q_blocks), block(p.rows == 1 ? 128 : 256);
+    const cudaError_t e = vec ? qs_launch_dependent(kv8_store_kernel<T, true>, grid, block, 0, stream, (T*)q_out, (const T*)q, (const T*)k, (const T*)v, (const T*)v_first, p)
+                              : qs_launch_dependent(kv8_store_kernel<T, false>, grid, block, 0, stream, (T*)q_out, (const T*)q, (const T*)k, (const T*)v, (const T*)v_first, p);
+    if (e != cudaSuccess) return qs_fail(QS_ERR_INTERNAL, "kv8 store: %s", cudaGetErrorString(e));
     return qs_check_launch("kv8 store");
 }
 
@@ -279,10 +443,15 @@ QS_API int qs_kv8_store(void* q_out, long long ldqo, const void* q, long long ld
     p.half_layout = half_layout; p.cos_sin = cos_sin;
     p.ldq = (size_t)ldq; p.ldqo = (size_t)ldqo; p.ldk = (size_t)ldk; p.ldv = (size_t)ldv; p.ldvf = (size_t)ldvf;
     p.k_cache = k_cache; p.v_cache = v_cache; p.k_scale = k_scale; p.v_scale = v_scale; p.status = status; p.lam = lam;
-    p.rows = T_tokens <= 256 ? 1 : 16;
+    // a row to a block while rows are few (a decode step: every row is a run of its own), else half a page
+    p.rows = T_tokens <= 256 ? 1 : 32;
+    const int e = dtype == QS_F32 ? 4 : 2;
+    auto pieces = [&](const void* x, long long ld) { return !x || (((uintptr_t)x % 16) == 0 && ld * e % 16 == 0); };
+    const bool vec = dk % 16 == 0 && dv % 16 == 0 && p.R % (half_layout ? 32 : 16) == 0 && pieces(q, ldq) && pieces(q_out, ldqo) && pieces(k, ldk) && pieces(v, ldv) &&
+                     ((uintptr_t)cos_sin % 16) == 0 && ((uintptr_t)k_cache % 16) == 0 && ((uintptr_t)v_cache % 16) == 0;
     const bool queries = q && n_heads > 0 && (p.R > 0 || q != q_out);
-    p.q_blocks = queries ? (int)(((long long)p.rows * n_heads * (dk / 2) + 1023) / 1024) : 0;
-    return dtype == QS_F32 ? store_launch<float>(q_out, q, k, v, v_first, p, stream) : store_launch<__nv_bfloat16>(q_out, q, k, v, v_first, p, stream);
+    p.q_blocks = queries ? (int)(((long long)p.rows * n_heads * dk / (vec ? 16 : 2) + 1023) / 1024) : 0;
+    return dtype == QS_F32 ? store_launch<float>(q_out, q, k, v, v_first, p, vec, stream) : store_launch<__nv_bfloat16>(q_out, q, k, v, v_first, p, vec, stream);
 }
 
 // out [n][n_kv_heads][64][dim] of type `dtype`: the numbers in the listed pages.
@@ -292,8 +461,14 @@ QS_API int qs_kv8_read_pages(void* out, int dtype, const int8_t* codes, const fl
     QS_REQUIRE(n > 0 && n <= 65535 && n_pages > 0 && n_kv_heads > 0 && dim > 0, "kv8 read_pages: %d pages of %d heads of %d", n, n_kv_heads, dim);
     QS_REQUIRE(dtype == QS_F32 || dtype == QS_BF16, "kv8 read_pages: type %d", dtype);
     const dim3 grid(n_kv_heads, n);
-    if (dtype == QS_F32) kv8_read_pages_kernel<float><<<grid, 256, 0, stream>>>((float*)out, codes, scales, pages, n_pages, n_kv_heads, dim);
-    else kv8_read_pages_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>((__nv_bfloat16*)out, codes, scales, pages, n_pages, n_kv_heads, dim);
+    const bool vec = dim % 4 == 0 && ((uintptr_t)codes % 16) == 0 && ((uintptr_t)out % 16) == 0;       // a page is 64 * dim codes
+    cudaError_t e;
+#define GO(T, VEC) e = qs_launch_dependent(kv8_read_pages_kernel<T, VEC>, grid, dim3(256), 0, stream, (T*)out, codes, scales, pages, n_pages, n_kv_heads, dim)
+    if (dtype == QS_F32) { if (vec) GO(float, true); else GO(float, false); }
+    else if (vec) GO(__nv_bfloat16, true);
+    else GO(__nv_bfloat16, false);
+#undef GO
+    if (e != cudaSuccess) return qs_fail(QS_ERR_INTERNAL, "kv8 read_pages: %s", cudaGetErrorString(e));
     return qs_check_launch("kv8 read_pages");
 }
 
