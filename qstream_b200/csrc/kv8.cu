@@ -107,32 +107,43 @@ __device__ __forceinline__ void rotated16(const T* __restrict__ row, int d, cons
     }
 }
 
-// Four numbers, already divided by the scale, as a word of codes.
-__device__ __forceinline__ uint32_t four_codes(float a, float b, float c, float d) {
-    const float v[4] = {a, b, c, d};
-    uint32_t r = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r |= (uint32_t)(max(-127, min(127, __float2int_rn(v[i]))) & 255) << (8 * i);
+// Four numbers times a power of two, at most 127 then, as a word of codes: added to 1.5 * 2^23 they are rounded to whole numbers (ties to even), whose
+// lowest byte the sum's is.
+__device__ __forceinline__ uint32_t four_codes(float a, float b, float c, float d, float factor) {
+    const float k = 12582912.f;
+    const uint32_t lo = __byte_perm(__float_as_uint(fmaf(a, factor, k)), __float_as_uint(fmaf(b, factor, k)), 0x0040);
+    const uint32_t hi = __byte_perm(__float_as_uint(fmaf(c, factor, k)), __float_as_uint(fmaf(d, factor, k)), 0x0040);
+    return __byte_perm(lo, hi, 0x5410);
+}
+
+// max(a, |b|), NaN where one is.
+__device__ __forceinline__ float max_size(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
     return r;
 }
 
 // n rows of one page and head, from row `a` of the page on: the scale that holds them and what is there already, then the codes.
 // VEC: value(i, d, x) gives elements d .. d + 15 of new row i, else element d.  The rows are read twice, the second time from the caches: they are too
 // many for the registers of a block, and the rotation is cheap.
+// Bound by the instructions as much as by memory: some fourteen for an element, seven of them its way through 32 bits and into the maximum, one and three
+// quarters its rounding and packing.
 template <bool VEC, typename F>
 __device__ __forceinline__ void store_run(int8_t* __restrict__ codes, float* __restrict__ scale, int a, int n, int dim, uint32_t* scratch, F value) {
     constexpr int E = VEC ? 16 : 1;
-    const int pieces = dim / E, items = n * pieces;
-    uint32_t most = 0;                                   // as bits: numbers that are not finite are above all others
-    for (int e = threadIdx.x; e < items; e += blockDim.x) {
+    const int pieces = dim / E, first = threadIdx.x / pieces, step = blockDim.x / pieces, at = threadIdx.x - first * pieces, more = blockDim.x - step * pieces;
+    float most = 0.f;
+    for (int i = first, c = at; i < n;) {
         float x[E];
-        value(e / pieces, e % pieces * E, x);
+        value(i, c * E, x);
 #pragma unroll
-        for (int i = 0; i < E; ++i) most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
+        for (int u = 0; u < E; ++u) most = max_size(most, x[u]);
+        i += step;
+        if ((c += more) >= pieces) { c -= pieces; ++i; }
     }
-    most = block_max(most, scratch);
+    const uint32_t bits = block_max(__float_as_uint(most), scratch);        // numbers that are not finite are above all others
     const float before = a > 0 ? *scale : 0.f;
-    const float need = most >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : most == 0 ? 0.f : scale_for(most);
+    const float need = bits >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : bits == 0 ? 0.f : scale_for(bits);
     const float after = isnan(before) || isnan(need) ? __uint_as_float(0x7fffffffu) : fmaxf(before, need);
     __syncthreads();                                     // everybody has read the old scale
     if (threadIdx.x == 0) *scale = after;
@@ -142,30 +153,32 @@ __device__ __forceinline__ void store_run(int8_t* __restrict__ codes, float* __r
             uint32_t* words = reinterpret_cast<uint32_t*>(codes);
             for (int e = threadIdx.x; e < a * dim / 4; e += blockDim.x) {
                 const uint32_t w = words[e];
-                words[e] = four_codes((float)(int8_t)w * shrink, (float)(int8_t)(w >> 8) * shrink, (float)(int8_t)(w >> 16) * shrink, (float)(int8_t)(w >> 24) * shrink);
+                words[e] = four_codes((float)(int8_t)w, (float)(int8_t)(w >> 8), (float)(int8_t)(w >> 16), (float)(int8_t)(w >> 24), shrink);
             }
         } else {
             for (int e = threadIdx.x; e < a * dim; e += blockDim.x) codes[e] = (int8_t)__float2int_rn((float)codes[e] * shrink);
         }
     }
-    const float inv = after > 0.f ? 1.0f / after : 0.f;  // NaN: the codes say nothing, and 0
-    for (int e = threadIdx.x; e < items; e += blockDim.x) {
+    const float inv = after > 0.f ? 1.0f / after : 0.f;
+    const bool nothing = !(inv > 0.f);                   // zeros; or NaN, and the codes say nothing: 0
+    for (int i = first, c = at; i < n;) {
         float x[E];
-        value(e / pieces, e % pieces * E, x);
+        value(i, c * E, x);
+        if (nothing) {
 #pragma unroll
-        for (int i = 0; i < E; ++i) x[i] = inv > 0.f ? x[i] * inv : 0.f;
-        if (VEC) {
-            constexpr int S = VEC ? 4 : 0;
-            *reinterpret_cast<uint4*>(codes + (size_t)a * dim + e * 16) =
-                make_uint4(four_codes(x[0], x[S / 4], x[S / 2], x[3 * S / 4]), four_codes(x[S], x[5 * S / 4], x[6 * S / 4], x[7 * S / 4]),
-                           four_codes(x[2 * S], x[9 * S / 4], x[10 * S / 4], x[11 * S / 4]), four_codes(x[3 * S], x[13 * S / 4], x[14 * S / 4], x[15 * S / 4]));
-        } else {
-            codes[(size_t)a * dim + e] = (int8_t)max(-127, min(127, __float2int_rn(x[0])));
+            for (int u = 0; u < E; ++u) x[u] = 0.f;
         }
+        int8_t* to = codes + (size_t)(a + i) * dim + c * E;
+        if constexpr (VEC)
+            *reinterpret_cast<uint4*>(to) = make_uint4(four_codes(x[0], x[1], x[2], x[3], inv), four_codes(x[4], x[5], x[6], x[7], inv),
+                                                       four_codes(x[8], x[9], x[10], x[11], inv), four_codes(x[12], x[13], x[14], x[15], inv));
+        else *to = (int8_t)__float2int_rn(x[0] * inv);
+        i += step;
+        if ((c += more) >= pieces) { c -= pieces; ++i; }
     }
 }
 
-// blockIdx.x: `rows` (up to 32) consecutive rows of the step; blockIdx.y: a key head, then blocks that rotate the queries of these rows.
+// blockIdx.x: `rows` (up to 32) consecutive rows of the step; blockIdx.y: a key head's keys, its values, ..., then blocks that rotate the queries of these rows.
 // A run is the rows of one sequence that fall into one page: consecutive rows of ascending positions.  The block of a run's first row takes
 // the whole run, so that a page's scale has one writer; a second run for the same page in one call is reported (status 5) and not written.
 // VEC: rows, angles and pages in pieces of 16 elements, on their boundaries.
@@ -178,11 +191,11 @@ kv8_store_kernel(T* q_out, const T* q, const T* __restrict__ k, const T* __restr
     grid_dep_wait();
     const int row0 = blockIdx.x * p.rows, rows = min(p.rows, p.T - row0), lane = threadIdx.x & 31;
     const bool rotate = p.cos_sin != nullptr && p.R > 0;
-    if ((int)blockIdx.y >= p.n_kv_heads) {
+    if ((int)blockIdx.y >= 2 * p.n_kv_heads) {
         // an item: 16 (VEC) or 1 pairs that turn, or as many plain elements of both halves of the rest
         const int rp = rotate ? p.R >> 1 : 0, turning = VEC && !p.half_layout ? rp / 8 : rp / E, plain = q_out == q ? 0 : (p.dk - 2 * rp) / E;
         const int per_head = turning + plain, per_row = p.n_heads * per_head, items = rows * per_row;
-        for (int e = (blockIdx.y - p.n_kv_heads) * blockDim.x + threadIdx.x; e < items; e += p.q_blocks * blockDim.x) {
+        for (int e = (blockIdx.y - 2 * p.n_kv_heads) * blockDim.x + threadIdx.x; e < items; e += p.q_blocks * blockDim.x) {
             const int i = e / per_row, r = row0 + i, rest = e - i * per_row, head = rest / per_head, j = rest - head * per_head;
             const int slot = p.tok_slot[r], pos = p.tok_pos[r];
             const bool fits = slot >= 0 && pos >= 0 && pos < p.max_pos;
@@ -235,13 +248,14 @@ kv8_store_kernel(T* q_out, const T* q, const T* __restrict__ k, const T* __restr
         }
         return;
     }
-    const int kvh = blockIdx.y;
+    const int kvh = blockIdx.y >> 1;
+    const bool keys = (blockIdx.y & 1) == 0, reports = blockIdx.y == 0 && threadIdx.x < 32;
     // which of the rows begin a run
     bool begins = false;
     if (lane < rows) {
         const int r = row0 + lane, slot = p.tok_slot[r], pos = p.tok_pos[r];
         const bool bad = slot >= p.n_slots || pos < 0 || (pos >> 6) >= p.max_pages || (rotate && pos >= p.max_pos);
-        if (slot >= 0 && bad && threadIdx.x < 32 && kvh == 0) atomicExch(p.status, 1);
+        if (slot >= 0 && bad && reports) atomicExch(p.status, 1);
         begins = slot >= 0 && !bad && !(r > 0 && (pos & (PAGE - 1)) != 0 && p.tok_slot[r - 1] == slot && p.tok_pos[r - 1] == pos - 1);
     }
     for (uint32_t todo = __ballot_sync(0xffffffffu, begins); todo != 0; todo &= todo - 1) {
@@ -249,7 +263,15 @@ kv8_store_kernel(T* q_out, const T* q, const T* __restrict__ k, const T* __restr
         const int page = p.page_table[(size_t)slot * p.max_pages + (pos >> 6)];
         if (page < 0 || page >= p.n_pages) { if (threadIdx.x == 0) atomicExch(p.status, 2); continue; }
         int again = 0;
-        for (int i = threadIdx.x; i < r; i += blockDim.x) again |= p.tok_slot[i] == slot && (p.tok_pos[i] >> 6) == (pos >> 6);
+        int whole = 0;                                   // rows looked at in fours
+        if ((((uintptr_t)p.tok_slot | (uintptr_t)p.tok_pos) & 15) == 0) {
+            whole = r & ~3;
+            for (int i = threadIdx.x; i < whole >> 2; i += blockDim.x) {
+                const int4 s4 = reinterpret_cast<const int4*>(p.tok_slot)[i], p4 = reinterpret_cast<const int4*>(p.tok_pos)[i];
+                again |= (s4.x == slot && p4.x >> 6 == pos >> 6) | (s4.y == slot && p4.y >> 6 == pos >> 6) | (s4.z == slot && p4.z >> 6 == pos >> 6) | (s4.w == slot && p4.w >> 6 == pos >> 6);
+            }
+        }
+        for (int i = whole + threadIdx.x; i < r; i += blockDim.x) again |= p.tok_slot[i] == slot && (p.tok_pos[i] >> 6) == (pos >> 6);
         const int a = pos & (PAGE - 1);
         // the run's length: the first row behind it, 64 rows looked at by two lanes' turns
         int n = PAGE - a;
@@ -262,13 +284,13 @@ kv8_store_kernel(T* q_out, const T* q, const T* __restrict__ k, const T* __restr
         }
         if (__syncthreads_or(again)) { if (threadIdx.x == 0) atomicExch(p.status, 5); continue; }
         const size_t at = (size_t)page * p.n_kv_heads + kvh;
-        store_run<VEC>(p.k_cache + at * PAGE * p.dk, p.k_scale + at, a, n, p.dk, scratch, [&](int i, int d, float (&x)[E]) {
+        if (keys) store_run<VEC>(p.k_cache + at * PAGE * p.dk, p.k_scale + at, a, n, p.dk, scratch, [&](int i, int d, float (&x)[E]) {
             const T* row = k + (size_t)(r + i) * p.ldk + (size_t)kvh * p.dk;
             const float* cs = p.cos_sin + (size_t)(pos + i) * p.R;
             if constexpr (VEC) rotated16(row, d, cs, rotate ? p.R : 0, p.half_layout, x);
             else x[0] = rotated(row, d, cs, rotate ? p.R : 0, p.half_layout);
         });
-        store_run<VEC>(p.v_cache + at * PAGE * p.dv, p.v_scale + at, a, n, p.dv, scratch, [&](int i, int d, float (&x)[E]) {
+        else store_run<VEC>(p.v_cache + at * PAGE * p.dv, p.v_scale + at, a, n, p.dv, scratch, [&](int i, int d, float (&x)[E]) {
             const T* row = v + (size_t)(r + i) * p.ldv + (size_t)kvh * p.dv + d;
             if constexpr (VEC) load16(row, x);
             else x[0] = to_f32(*row);
@@ -404,7 +426,7 @@ kv8_attention_kernel(TO* __restrict__ out, const T* __restrict__ q, const Attend
 
 template <typename T>
 int store_launch(void* q_out, const void* q, const void* k, const void* v, const void* v_first, const StoreArgs& p, bool vec, cudaStream_t stream) {
-    const dim3 grid((p.T + p.rows - 1) / p.rows, p.n_kv_heads + p.q_blocks), block(p.rows == 1 ? 128 : 256);
+    const dim3 grid((p.T + p.rows - 1) / p.rows, 2 * p.n_kv_heads + p.q_blocks), block(p.rows == 1 ? 128 : 256);
     const cudaError_t e = vec ? qs_launch_dependent(kv8_store_kernel<T, true>, grid, block, 0, stream, (T*)q_out, (const T*)q, (const T*)k, (const T*)v, (const T*)v_first, p)
                               : qs_launch_dependent(kv8_store_kernel<T, false>, grid, block, 0, stream, (T*)q_out, (const T*)q, (const T*)k, (const T*)v, (const T*)v_first, p);
     if (e != cudaSuccess) return qs_fail(QS_ERR_INTERNAL, "kv8 store: %s", cudaGetErrorString(e));
@@ -435,7 +457,7 @@ QS_API int qs_kv8_store(void* q_out, long long ldqo, const void* q, long long ld
     QS_REQUIRE(dk > 0 && dk % 2 == 0 && dk <= 512 && dv > 0 && dv <= 512, "kv8 store: head sizes %d and %d (keys: even; up to 512)", dk, dv);
     QS_REQUIRE(!cos_sin || (R >= 0 && R % 2 == 0 && R <= dk && max_pos > 0), "kv8 store: %d rotated dims of %d", R, dk);
     QS_REQUIRE(dtype == QS_F32 || dtype == QS_BF16, "kv8 store: type %d", dtype);
-    QS_REQUIRE(n_kv_heads <= 32768, "kv8 store: %d key heads exceed the grid", n_kv_heads);
+    QS_REQUIRE(n_kv_heads <= 16384, "kv8 store: %d key heads exceed the grid", n_kv_heads);
     StoreArgs p = {};
     p.tok_slot = tok_slot; p.tok_pos = tok_pos; p.page_table = page_table;
     p.T = T_tokens; p.max_pages = max_pages; p.n_slots = n_slots; p.n_pages = n_pages;
