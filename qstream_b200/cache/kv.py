@@ -14,13 +14,17 @@ last page, by weights of exactly zero, and 0 * Inf is NaN.  So a page that held 
 sequence's values is zeroed when it is handed on, unless the step that takes it writes
 all of its rows.
 
+A cache of type int8 holds codes, and beside them a float32 scale for each entry, page and head (K and V apart):
+a number is code * scale (csrc/kv8.py).  A page's scale starts afresh with the token in its first row, and codes are
+finite whatever they stand for, so no page needs to be zeroed.
+
 This replaces QStream's single-sequence cache (`QSFKVCache`, include/qsf/engine.h:35-51,
-src/engine.c:296-327; `current_seq_len`), whose int8 storage is not taken over.
+src/engine.c:296-327; `current_seq_len`), which holds int8 codes with a scale per position.
 """
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Mapping, Sequence
+from typing import Mapping, Optional, Sequence
 
 import numpy as np
 import torch
@@ -71,6 +75,8 @@ class CacheView:
     page_table: torch.Tensor            # [slots, max_pages] int32, device
     page_tokens: int
     need: KvNeed
+    k_scale: Optional[torch.Tensor] = None      # [pages, kv_heads] float32 where k and v hold 8-bit codes
+    v_scale: Optional[torch.Tensor] = None
 
 
 class KvGroup:
@@ -87,6 +93,8 @@ class KvGroup:
         # the end are replaced, not multiplied) when it is handed on to a step that leaves rows unwritten.
         self.k = torch.zeros(shape, dtype=dtype, device=device)
         self.v = torch.zeros((*shape[:-1], need.value_dim), dtype=dtype, device=device)
+        self.k_scale = torch.zeros(shape[:3], dtype=torch.float32, device=device) if dtype == torch.int8 else None
+        self.v_scale = torch.zeros(shape[:3], dtype=torch.float32, device=device) if dtype == torch.int8 else None
         self._used = np.zeros(n_pages, dtype=bool)
         self._to_zero: list[int] = []
         self.table_host = np.full((n_slots, max_pages), -1, dtype=np.int32)
@@ -98,9 +106,12 @@ class KvGroup:
         self.n_pages = n_pages
         if self.k.is_cuda:
             from ..csrc import ops
-            for store in (self.k, self.v):
+            for store in self._stores():
                 for e in range(len(self.entries)):
                     ops.canary_fill(store[e, n_pages], CANARY)
+
+    def _stores(self) -> list:
+        return [t for t in (self.k, self.v, self.k_scale, self.v_scale) if t is not None]
 
     def damaged_guard_words(self) -> int:
         """How many guard words behind the entries' pages no longer hold their pattern (0 on a host cache)."""
@@ -108,14 +119,14 @@ class KvGroup:
             return 0
         from ..csrc import ops
         damaged = torch.zeros(2, dtype=torch.int32, device=self.k.device)
-        for store in (self.k, self.v):
+        for store in self._stores():
             for e in range(len(self.entries)):
                 ops.canary_check(store[e, self.n_pages], CANARY, damaged)
         return int(damaged[0].item())
 
     @property
     def bytes(self) -> int:
-        return (self.k.numel() + self.v.numel()) * self.k.element_size()
+        return sum(t.numel() * t.element_size() for t in self._stores())
 
     def pages_needed(self, slot: int, new_length: int) -> int:
         return max(0, -(-new_length // self.page_tokens) - self.first_page[slot] - self.held[slot])
@@ -129,7 +140,7 @@ class KvGroup:
         row = self.table_host[slot]
         for i in range(have, n):
             page = row[i] = self.pool.alloc()
-            if self._used[page] and new_length < (i + 1) * self.page_tokens:
+            if self._used[page] and new_length < (i + 1) * self.page_tokens and self.k_scale is None:
                 self._to_zero.append(page)          # used before, and this step does not fill it
             self._used[page] = True
         self.held[slot] += n - have
@@ -185,7 +196,8 @@ class KvGroup:
 
     def view(self, cache_id: int) -> CacheView:
         e = self.entries.index(cache_id)
-        return CacheView(self.k[e], self.v[e], self.table_dev, self.page_tokens, self.need)
+        scales = (None, None) if self.k_scale is None else (self.k_scale[e], self.v_scale[e])
+        return CacheView(self.k[e], self.v[e], self.table_dev, self.page_tokens, self.need, *scales)
 
 
 class StateStore:

@@ -10,7 +10,8 @@ prompt is a list of token ids ("5,17,3"; several requests separated by ';' or gi
 repeated -p, or one per line in --prompt-file), and the chat options are gone.  New:
 --dtype, --max-batch, --max-ctx, --stop-token (repeatable; "none" for no stop token),
 --random-weights SEED with --config FILE (writes nothing; weights are made on the device),
---check-nan (scan every layer's output for values that are not finite, as the reference's
+--weight-bits 4 (matrices of attention and dense feed-forwards in 4 bits), --weight-group (columns to a scale, 64),
+--cache-dtype int8 (keys and values in 8 bits), --check-nan (scan every layer's output for values that are not finite, as the reference's
 `check_nan` switch does, include/qsf/engine.h:31).
 Generated ids go to standard output, one request per line; statistics to standard error as
 in src/main.c:323-332.
@@ -63,6 +64,9 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--config", help="config.json for --random-weights")
     ap.add_argument("--narrow-fp32", action="store_true",
                     help="with --dtype bfloat16: round matrices stored in 32-bit to bfloat16 (default: they stay 32-bit)")
+    ap.add_argument("--weight-bits", type=int, choices=[4], help="hold the matrices of attention and dense feed-forwards in 4 bits")
+    ap.add_argument("--weight-group", type=int, default=64, help="with --weight-bits: columns that share a scale (32, 64 or 128; default: 64)")
+    ap.add_argument("--cache-dtype", default="", choices=["", "int8"], help="hold keys and values in 8 bits (default: the --dtype)")
     ap.add_argument("--check-nan", action="store_true", help="check every layer's output for NaN/Inf (slow)")
     return ap
 
@@ -91,19 +95,20 @@ def main(argv=None) -> int:
                 return 1
             with open(args.config) as fh:
                 cfg = config_from_dict(json.load(fh))
-            model = qs.CausalLM.random(cfg, args.random_weights, args.dtype, "cuda")
+            model = qs.CausalLM.random(cfg, args.random_weights, args.dtype, "cuda", weight_bits=args.weight_bits, weight_group=args.weight_group)
         else:
             model = qs.load_model(args.model, dtype=args.dtype, device="cuda", allow_mmap=not args.no_mmap,
-                                  narrow_fp32_matrices=args.narrow_fp32)
+                                  narrow_fp32_matrices=args.narrow_fp32,
+                                  weight_bits=args.weight_bits, weight_group=args.weight_group)
         ctx = args.max_ctx or model.spec.max_positions
         max_batch = max(1, min(args.max_batch, len(prompts)))
         max_tokens = max_batch * (-(-min(ctx, model.spec.max_positions) // 64) * 64)
         if args.ram_budget:
             per_token = sum(n.n_kv_heads * (n.head_dim + n.value_dim) for n in model.kv_needs().values()) * \
-                torch.empty((), dtype=model.runtime.dtype).element_size()
+                torch.empty((), dtype=torch.int8 if args.cache_dtype else model.runtime.dtype).element_size()
             max_tokens = min(max_tokens, max(64, args.ram_budget * 2**20 // max(per_token, 1) // 64 * 64))
         engine = qs.Engine(model, qs.EngineConfig(max_tokens=max_tokens, max_batch=max_batch, max_context=ctx,
-                                                  verbose=args.verbose, check_nan=args.check_nan))
+                                                  verbose=args.verbose, check_nan=args.check_nan, cache_dtype=args.cache_dtype))
         if args.verbose:
             print(f"[qstream] model loaded in {(time.perf_counter() - t0) * 1e3:.1f} ms "
                   f"({model.n_parameters / 1e6:.1f} M parameters, {args.dtype})", file=sys.stderr)

@@ -17,7 +17,7 @@ import torch
 
 from ..cache import KvNeed, StateNeed
 from ..config import ModelSpec, load_config
-from ..csrc import ops
+from ..csrc import ops, q4
 from ..errors import QsError, QStreamError
 from ..parts import Runtime, build_block, part_class
 from ..weights.loader import TensorDecl, bind_tensors, open_checkpoint
@@ -66,10 +66,16 @@ def declared_tensors(spec: ModelSpec) -> dict[str, TensorDecl]:
 class CausalLM:
     """Parts, weights and the forward pass of one model."""
 
-    def __init__(self, spec: ModelSpec, tensors: Mapping[str, torch.Tensor], dtype, device, config=None):
+    def __init__(self, spec: ModelSpec, tensors: Mapping[str, torch.Tensor], dtype, device, config=None, weight_bits=None, weight_group=64):
+        """`weight_bits` 4: the matrices of attention and dense feed-forwards are rounded to 4 bits, with a bfloat16 scale for
+        each row and `weight_group` columns (32, 64 or 128); None: every tensor as it is stored."""
         self.spec = spec
         self.config = config
-        self.runtime = Runtime(dtype=resolve_dtype(dtype), device=torch.device(device))
+        if weight_bits not in (None, 4):
+            raise QStreamError(QsError.QUANT_MISMATCH, f"weights of {weight_bits} bits: want 4, or None for the stored type")
+        if weight_bits == 4 and weight_group not in q4.GROUPS:
+            raise QStreamError(QsError.QUANT_MISMATCH, f"weights of 4 bits in groups of {weight_group} columns (groups: {q4.GROUPS})")
+        self.runtime = Runtime(dtype=resolve_dtype(dtype), device=torch.device(device), weight_group=int(weight_group) if weight_bits == 4 else 0)
         self.vocab_size = spec.vocab_size
 
         def tensors_of(part_spec, decls):
@@ -89,6 +95,9 @@ class CausalLM:
         self._check_schedule()
         self.n_parameters = sum(t.numel() for t in {id(t): t for t in tensors.values()}.values())
         self.weight_bytes = sum(t.numel() * t.element_size() for t in {id(t): t for t in tensors.values()}.values())
+        self.weight_bytes -= sum(before - after for before, after in self.runtime.narrowed)
+        if weight_bits == 4 and not self.runtime.narrowed:
+            raise QStreamError(QsError.UNSUPPORTED_ARCH, "weights of 4 bits: no layer of this model has a matrix that is held so")
 
     @property
     def embedding_bytes(self) -> int:
@@ -100,10 +109,11 @@ class CausalLM:
     # ------------------------------------------------------------------ making a model
     @classmethod
     def from_folder(cls, folder, dtype="bfloat16", device="cuda", allow_mmap=True, verbose=0,
-                    narrow_fp32_matrices=False):
+                    narrow_fp32_matrices=False, weight_bits=None, weight_group=64):
         """config.json chooses the architecture; *.safetensors give the weights.
         narrow_fp32_matrices: round matrices that the files store in 32-bit to bfloat16 in a
-        bfloat16 engine (default: a tensor stored in 32-bit stays in 32-bit)."""
+        bfloat16 engine (default: a tensor stored in 32-bit stays in 32-bit).  weight_bits, weight_group: as for
+        the constructor."""
         config = load_config(folder)
         spec = config.model_spec()
         files = open_checkpoint(folder, allow_mmap)
@@ -114,14 +124,14 @@ class CausalLM:
         finally:
             for f in files:
                 f.close()
-        return cls(spec, tensors, dtype, device, config)
+        return cls(spec, tensors, dtype, device, config, weight_bits, weight_group)
 
     @classmethod
-    def random(cls, config, seed=0, dtype="bfloat16", device="cuda", scales: InitScales = InitScales()):
+    def random(cls, config, seed=0, dtype="bfloat16", device="cuda", scales: InitScales = InitScales(), weight_bits=None, weight_group=64):
         """Random weights made on the device, without a model folder."""
         spec = config.model_spec()
         tensors = random_tensors(declared_tensors(spec), seed, resolve_dtype(dtype), device, scales)
-        return cls(spec, tensors, dtype, device, config)
+        return cls(spec, tensors, dtype, device, config, weight_bits, weight_group)
 
     # ------------------------------------------------------------------ what the cache must hold
     def _cache_users(self):
@@ -152,6 +162,11 @@ class CausalLM:
                 if cid not in writers or writers[cid] > i:
                     raise QStreamError(QsError.INVALID_MODEL,
                                        f"schedule entry {i} reads cache entry {cid} before any layer wrote it")
+
+    def takes_cache8(self) -> bool:
+        """Whether every part that keeps or reads keys and values runs over a cache of 8-bit codes."""
+        return all(getattr(part, "takes_cache8", False) for _, _, part in self._cache_users()
+                   if part.kv_need() is not None or getattr(part.spec, "shares_cache", False))
 
     def kv_needs(self) -> dict[int, KvNeed]:
         return {cid: part.kv_need() for _, cid, part in self._cache_users() if part.kv_need() is not None}

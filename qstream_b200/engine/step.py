@@ -65,7 +65,9 @@ class EngineConfig:
     mem_budget: bytes of device memory the cache may take (0: what is free).  check_nan: scan
     every layer's output for values that are not finite and raise NAN_DETECTED with the layer
     and the place (the reference's switch, src/engine.c:1176-1187); it makes every step wait
-    for the device.  use_graphs: replay decode steps as CUDA graphs."""
+    for the device.  use_graphs: replay decode steps as CUDA graphs.  cache_dtype: "" for a
+    cache of the engine's type; "int8" for keys and values as 8-bit codes with a scale for each page and key head,
+    half of the bytes in the bfloat16 engine and a quarter in the float32 one (models whose mixers all offer it)."""
     max_batch: int = 64
     max_context: int = 0
     max_tokens: int = 0
@@ -73,6 +75,7 @@ class EngineConfig:
     verbose: int = 0
     check_nan: bool = False
     use_graphs: bool = True
+    cache_dtype: str = ""
 
     @classmethod
     def default(cls) -> "EngineConfig":
@@ -117,6 +120,7 @@ STATUS_MESSAGES = {
     1: "a token's position lies outside the position table",
     2: "a token was to be written to a cache page its sequence does not hold",
     3: "attention met a cache page its sequence does not hold",
+    5: "a sequence's tokens for one cache page lay apart in a step",
     199: "the self-test's wait ran out, as it must",
 }
 
@@ -144,8 +148,14 @@ class Engine:
         max_tokens = cfg.max_tokens or max_batch * ctx
         self.max_batch = max_batch
         kv_needs, state_needs = model.kv_needs(), model.state_needs()
-        self._check_budget(kv_needs, max_tokens, cfg.mem_budget)
-        self.cache = SequenceCache(kv_needs, state_needs, max_tokens, max_batch, ctx, self.dtype, self.device)
+        if cfg.cache_dtype not in ("", "int8"):
+            raise QStreamError(QsError.INVALID_INPUT, f"Engine: a cache of type '{cfg.cache_dtype}' (want 'int8', or '' for the engine's)")
+        if cfg.cache_dtype and not (kv_needs and model.takes_cache8()):
+            raise QStreamError(QsError.UNSUPPORTED_ARCH, "Engine: a layer of this model does not run over an 8-bit cache" if kv_needs else
+                               "Engine: this model keeps no keys and values to hold in 8 bits")
+        cache_dtype = torch.int8 if cfg.cache_dtype else self.dtype
+        self._check_budget(kv_needs, max_tokens, cfg.mem_budget, cache_dtype)
+        self.cache = SequenceCache(kv_needs, state_needs, max_tokens, max_batch, ctx, cache_dtype, self.device)
         # words the kernels report through: [0] a fault code, [4:8] the finite check's record
         self._words = torch.zeros(8, dtype=torch.int32, device=self.device)
         self.status = self._words[0:1]
@@ -168,9 +178,11 @@ class Engine:
                   f"{self.cache.slots.n_slots} slots, context {ctx}; weights {model.weight_bytes / 2**20:.1f} MB",
                   file=sys.stderr)
 
-    def _check_budget(self, kv_needs, max_tokens, mem_budget=0):
-        elem = torch.empty((), dtype=self.dtype).element_size()
+    def _check_budget(self, kv_needs, max_tokens, mem_budget=0, cache_dtype=None):
+        elem = torch.empty((), dtype=cache_dtype or self.dtype).element_size()
         want = sum(max_tokens * n.n_kv_heads * (n.head_dim + n.value_dim) * elem for n in kv_needs.values())
+        if cache_dtype == torch.int8:                       # two scales to a page of 64 tokens and head
+            want += sum(-(-max_tokens // 64) * n.n_kv_heads * 8 for n in kv_needs.values())
         if mem_budget and want > mem_budget:
             raise QStreamError(QsError.BUDGET_EXCEEDED,
                                f"a cache of {max_tokens} tokens needs {want / 2**20:.1f} MiB, "

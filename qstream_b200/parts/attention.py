@@ -15,6 +15,9 @@ only inside the query's chunk of positions, or inside a window that also keeps t
 sink per head in the softmax's denominator; two attention maps per head over the same values, joined as a difference
 with a unit RMS per head (differential attention); one RMS norm over the whole q and the whole k projection before the
 heads are split, or a unit RMS per head behind the rotation; values that are the keys as projected (no W_v); a sink of a fixed score without a tensor.
+
+Over a cache of 8-bit codes (`csrc.kv8`) the rotation, the blend of values and the cache write are one kernel as well; the maps per
+head and the norms of q and k are not offered there.
 """
 from __future__ import annotations
 
@@ -89,7 +92,7 @@ class Attention(Mixer):
             mats.append(torch.zeros((pad, spec.width), dtype=mats[0].dtype, device=mats[0].device))
         if len({m.dtype for m in mats}) != 1:
             raise QStreamError(QsError.INVALID_MODEL, "q/k/v projections are stored in different types")
-        self.w_qkv = torch.cat(mats, dim=0).contiguous() if len(mats) > 1 else mats[0]
+        self.w_qkv = runtime.matrix(torch.cat(mats, dim=0).contiguous() if len(mats) > 1 else mats[0])
         self.b_qkv = None
         if spec.qkv_bias:
             biases = [tensors[n + "_bias"].float() for n in names]
@@ -98,7 +101,7 @@ class Attention(Mixer):
             self.b_qkv = torch.cat(biases).contiguous()
         # the blend's weight is a constant of the model: read once, passed to the kernel by value
         self.value_mix = float(tensors["value_mix"].float().item()) if spec.value_mix == "blend" else 0.0
-        self.w_out = tensors["out"]
+        self.w_out = runtime.matrix(tensors["out"])
         self.b_out = tensors.get("out_bias") if spec.out_bias else None
         self.maps = int(getattr(spec, "maps", 1))
         self.chunk, self.keep_first = int(getattr(spec, "chunk", 0)), int(getattr(spec, "keep_first", 0))
@@ -128,6 +131,10 @@ class Attention(Mixer):
     def cache_bytes_per_key(self) -> int:
         """What one key of a sequence costs a decode step to read: its key and its value, all heads."""
         return self.spec.n_kv_heads * (self.maps * self.spec.head_dim + self.spec.value_dim) * self.w_qkv.element_size()
+
+    @property
+    def takes_cache8(self) -> bool:
+        return self.maps == 1 and self.qk_norm is None
 
     def kv_need(self):
         if self.spec.shares_cache:
@@ -163,6 +170,8 @@ class Attention(Mixer):
         if s.gate and out is not None:
             raise QStreamError(QsError.INVALID_INPUT, "attention: a gated mixer writes its own output")
         half = bool(getattr(self.position, "half_layout", False))
+        if view.k_scale is not None:
+            return self._forward_codes(q, qkv, step, view, out, table, half)
         if self.maps > 1 and self.position is not None:
             raise QStreamError(QsError.UNSUPPORTED_ARCH, "attention: several maps per head with a rotation")
         if self.qk_norm == "head":                      # rotation, a unit RMS per head and the cache write as one kernel
@@ -215,6 +224,51 @@ class Attention(Mixer):
         if not self.masked:
             return attend(q, s, step, view, out, gate=gate)
         return self._attend_masked(q, step, view, out, gate)
+
+    def _forward_codes(self, q, qkv, step, view, out, table, half):
+        """`forward_hidden` behind the projections, over a cache of 8-bit codes."""
+        from ..csrc import attention_bf16, kv8
+        s, b = self.spec, step.batch
+        hq, hkv, hv = s.n_heads * s.head_dim, s.n_kv_heads * s.head_dim, s.n_kv_heads * s.value_dim
+        if not self.takes_cache8:
+            raise QStreamError(QsError.UNSUPPORTED_ARCH, "attention: several maps per head or norms of q and k over an 8-bit cache")
+        rotary = self.position.rotary_dim if table is not None else 0
+        cache = (view.page_table, view.page_tokens, view.k, view.v, view.k_scale, view.v_scale)
+        k = None if s.shares_cache else qkv[:, hq:hq + hkv]
+        v = None
+        if k is not None:
+            v = k if self.values_from_keys else qkv[:, hq + hkv:hq + hkv + hv]
+        if self.position is not None and table is None:
+            if self.values_from_keys and k is not None:
+                v = v.clone()                               # the keys as projected, before they are rotated in place
+            self.position.apply(q, k, step, s.n_heads, s.n_kv_heads, s.head_dim)
+        if k is None:
+            if table is not None:                           # rotate q only: no keys of its own
+                ops.rope_store(q, None, None, s.n_heads, 0, s.head_dim, rotary, table, b.tok_slot, b.tok_pos, None, view.page_tokens, None, None,
+                               step.status, settled=True, half_layout=half)
+        else:
+            v_first = None
+            if s.value_mix == "first":
+                step.scratch["value_mix"] = v               # later layers of this step blend their values with these
+            elif s.value_mix == "blend":
+                v_first = step.scratch.get("value_mix")
+                if v_first is None or v_first.shape != v.shape:
+                    raise QStreamError(QsError.INVALID_MODEL, "attention: values to blend with, but no earlier layer kept any of this shape")
+            kv8.rope_store(q, k, v, s.n_heads, s.n_kv_heads, s.head_dim, rotary, table, b.tok_slot, b.tok_pos, *cache, step.status,
+                           v_head_dim=s.value_dim, v_first=v_first, v_mix=self.value_mix, half_layout=half)
+        gate = qkv[:, self.gate_at:self.gate_at + self.gate_rows] if s.gate else None
+        opts = dict(out=None if gate is not None else out, v_head_dim=s.value_dim, softcap=s.softcap, chunk=self.chunk, keep_first=self.keep_first, sink=self.sink)
+        shape = (s.n_heads, s.n_kv_heads, s.head_dim, s.scale, s.window)
+        if b.decode:
+            # as for a bfloat16 cache: the longest sequence of the step, or the bound that a captured step was captured for
+            reach = min(b.max_total or step.cache.max_context, step.cache.max_context)
+            o = kv8.decode(q, *shape, b.tok_slot, b.tok_pos, *cache, reach, step.status, **opts)
+        else:
+            tiles = attention_bf16.prefill_tiles(b, q.device)
+            o = kv8.prefill(q, *shape, tiles, *cache, step.status, padded=b.n_tokens != sum(b.new_tokens), **opts)
+        if gate is not None:
+            o = ops.gated_group_norm(o, 0, None, gate, "sigmoid", 0.0, o.dtype, gate_span=s.value_dim if s.gate == "head" else 1)
+        return o
 
     def _attend_masked(self, q, step, view, out, gate):
         """Chunks, kept first tokens, sinks and pairs of maps: the bfloat16 engine's decode and prefill kernels take

@@ -32,7 +32,7 @@ rounding to the storage type; a part that cannot do that in its last kernel call
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import Mapping, Optional
 
 import torch
@@ -65,6 +65,17 @@ class Runtime:
     """Where and in which precision the parts compute."""
     dtype: torch.dtype                  # storage type of activations: bfloat16 or float32
     device: torch.device
+    weight_group: int = 0               # g > 0: the matrices of attention and dense feed-forwards in 4 bits, a scale for each g columns
+    narrowed: list = field(default_factory=list)        # (bytes before, bytes after) of every matrix that `matrix` rounded
+
+    def matrix(self, weight: torch.Tensor):
+        """A part's matrix as its products take it: as it is, or rounded to 4 bits."""
+        if not self.weight_group:
+            return weight
+        from ..csrc import q4
+        narrow = q4.quantize(weight, self.weight_group)
+        self.narrowed.append((weight.numel() * weight.element_size(), narrow.nbytes))
+        return narrow
 
 
 class Part:
@@ -112,6 +123,7 @@ class PositionEncoding(Part):
 
 class Mixer(Part):
     role = "mixer"
+    takes_cache8 = False                # whether it runs over a cache of 8-bit codes (an instance may know better than its class)
 
     def kv_need(self) -> Optional[KvNeed]:
         return None

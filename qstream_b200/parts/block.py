@@ -95,7 +95,8 @@ class ParallelBlock(Arrangement):
         self.fused_weight = None
         import torch
         fusable = all(hasattr(p, "output_projection") and hasattr(p, "forward_hidden") for p in (self.mixer, self.ffn))
-        if fusable and runtime.dtype == torch.bfloat16:
+        # (matrices in 4 bits stay apart: the products take one matrix with one layout of groups)
+        if fusable and not runtime.weight_group and runtime.dtype == torch.bfloat16:
             (wm, bm), (wf, bf) = self.mixer.output_projection(), self.ffn.output_projection()
             if (wm.dtype == wf.dtype == torch.bfloat16 and wm.shape[0] == wf.shape[0]
                     and wm.shape[1] % 8 == 0 and wf.shape[1] % 8 == 0):

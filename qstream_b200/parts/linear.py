@@ -6,6 +6,8 @@ number as three bfloat16 terms and the sums rounded in 32 bits outside the unit,
 sum of 256 products or more and rows come in 16-byte pieces; everything else (short sums, mixed types)
 runs on the CUDA cores in true 32-bit.
 
+A matrix may also be held in 4 bits (`csrc.q4.Weight4`); its products take both types of activations.
+
 A row's result does not depend on the contents of the other rows.  Neither does it depend on their number in
 the float32 engine, where the matrix alone decides the kernel and the order of the sums; the bfloat16
 products change their order between up to 128 rows and more (and with the number beyond), by rounding.
@@ -14,7 +16,8 @@ from __future__ import annotations
 
 import torch
 
-from ..csrc import ops
+from ..csrc import ops, q4
+from ..csrc.q4 import Weight4
 
 TENSOR_CORE_ACTIVATIONS = (None, "none", "gelu_new", "gelu")
 # float32: from how many products per result on the tensor cores serve, whatever the number of rows, so that a row's result is the same bits in any
@@ -29,6 +32,8 @@ OWN_KERNEL_ACTIVATIONS = ("relu2",)         # in no product's epilogue: applied 
 def linear(x, weight, bias=None, activation=None, residuals=(), out_dtype=None, out=None) -> torch.Tensor:
     """`out`: an optional view [M, N] with contiguous rows (any row stride) to write into."""
     residuals = tuple(r for r in residuals if r is not None)
+    if isinstance(weight, Weight4):
+        return q4.linear(x, weight, bias, activation, residuals, out_dtype, out, settled=True)
     if x.dtype == torch.bfloat16 and weight.dtype == torch.bfloat16:
         from ..csrc import gemm_tc
         if gemm_tc.takes(x, weight):

@@ -26,7 +26,7 @@ class Mlp(FeedForward):
         super().__init__(spec, tensors, runtime)
         if spec.activation not in ops.ACTIVATIONS:
             raise QStreamError(QsError.UNSUPPORTED_ARCH, f"activation '{spec.activation}' has no kernel")
-        self.up, self.down = tensors["up"], tensors["down"]
+        self.up, self.down = runtime.matrix(tensors["up"]), runtime.matrix(tensors["down"])
         self.up_bias = tensors.get("up_bias") if spec.bias else None
         self.down_bias = tensors.get("down_bias") if spec.bias else None
 
@@ -63,8 +63,8 @@ class GatedMlp(FeedForward):
         import torch
         if spec.activation not in ops.ACTIVATIONS:
             raise QStreamError(QsError.UNSUPPORTED_ARCH, f"activation '{spec.activation}' has no kernel")
-        self.gate_up = torch.cat([tensors["gate"], tensors["up"]], dim=0).contiguous()
-        self.down = tensors["down"]
+        self.gate_up = runtime.matrix(torch.cat([tensors["gate"], tensors["up"]], dim=0).contiguous())
+        self.down = runtime.matrix(tensors["down"])
         self.gate_up_bias = self.down_bias = None
         if getattr(spec, "bias", False):
             self.gate_up_bias = torch.cat([tensors["gate_bias"].float(), tensors["up_bias"].float()]).contiguous()
