@@ -10,7 +10,16 @@
 #include "per_device.h"
 #include "sm100.cuh"
 
+// For many bfloat16 rows (q4_many.cu).
+int q4_linear_many(void* out, int out_dtype, long long ldo, const void* x, long long ldx, const void* codes, const void* scales, const void* bias, int bias_dtype,
+                   int act, const void* res0, const void* res1, long long ldr, int M, int N, int chunks, int group, int settled, void* scratch, int32_t* status,
+                   cudaStream_t stream);
+long long q4_many_scratch(int M, int N, int chunks);
+
 namespace {
+
+// From how many bfloat16 rows on the products go to the 5th-generation tensor cores.
+constexpr int MANY_ROWS = 17;
 
 // The column within eight of a word's i-th code.
 __device__ __forceinline__ int column_of(int i) { return i < 4 ? 2 * i : 2 * i - 7; }
@@ -348,19 +357,25 @@ QS_API int qs_q4_quantize(void* codes, void* scales, const void* w, int dtype, l
     return qs_check_launch("q4 quantize");
 }
 
-// Bytes of workspace that `qs_q4_linear` takes for rows laid out anew; 0 where it takes them as they are.
-QS_API long long qs_q4_linear_scratch(int M, int K, int dtype, int aligned) {
+// Bytes of the rows laid out anew; 0 where the products take them as they are.
+static long long rows_scratch(int M, int K, int dtype, int aligned) {
     const int columns = (K + 63) / 64 * 64;
     if (dtype == QS_BF16 && aligned && K == columns) return 0;
     return (long long)M * (dtype == QS_F32 ? 3 : 1) * columns * 2;
 }
 
+// Bytes of workspace that `qs_q4_linear` takes, and its kernels.
+QS_API long long qs_q4_linear_scratch(int M, int N, int K, int dtype, int aligned) {
+    return rows_scratch(M, K, dtype, aligned) + (dtype == QS_BF16 && M >= MANY_ROWS ? q4_many_scratch(M, N, (K + 63) / 64) : 0);
+}
+QS_API int qs_q4_linear_kernels(int M, int K, int dtype, int aligned) { return 1 + (rows_scratch(M, K, dtype, aligned) > 0) + (dtype == QS_BF16 && M >= MANY_ROWS); }
+
 // out [M, N] = act(x W^T + bias) + residuals; x of type `dtype`, out of type `out_dtype` (float32 for float32 rows).  `aligned`: rows of x begin on
 // 16-byte boundaries.  `settled`: codes and scales were complete before the previous kernel of the stream began; the kernel then reads them while that kernel
-// still runs.  `scratch`: qs_q4_linear_scratch bytes on a 16-byte boundary.
+// still runs.  `scratch`: qs_q4_linear_scratch bytes on a 16-byte boundary.  `status`: set to a code of 130 and more if a wait inside the kernel ran out.
 QS_API int qs_q4_linear(void* out, int out_dtype, long long ldo, const void* x, int dtype, long long ldx, int aligned, const void* codes, const void* scales,
                         const void* bias, int bias_dtype, int act, const void* res0, const void* res1, long long ldr, int M, int N, int K, int group,
-                        int settled, void* scratch, cudaStream_t stream) {
+                        int settled, void* scratch, int32_t* status, cudaStream_t stream) {
     if (M == 0) return QS_OK;
     QS_REQUIRE(M > 0 && N > 0 && K > 0 && (group == 32 || group == 64 || group == 128), "q4 linear: [%d, %d] times [%d, %d] in groups of %d", M, K, N, K, group);
     QS_REQUIRE(((uintptr_t)codes % 16) == 0 && ((uintptr_t)scales % 4) == 0, "q4 linear: codes off their 16-byte boundary");
@@ -371,7 +386,8 @@ QS_API int qs_q4_linear(void* out, int out_dtype, long long ldo, const void* x, 
     QS_REQUIRE(!aligned || (((uintptr_t)x % 16) == 0 && ldx * e % 16 == 0), "q4 linear: rows off their 16-byte boundaries");
     Few p = {out, (const __nv_bfloat16*)x, bias, res0, res1, (const uint4*)codes, (const uint32_t*)scales, (size_t)ldo, (size_t)ldx, (size_t)ldr,
              M, N, chunks, 0, dtype == QS_F32 ? 3 : 1, out_dtype, dtype, bias_dtype, act, settled};
-    if (qs_q4_linear_scratch(M, K, dtype, aligned) > 0) {
+    const long long rows = rows_scratch(M, K, dtype, aligned);
+    if (rows > 0) {
         QS_REQUIRE(scratch && ((uintptr_t)scratch % 16) == 0, "q4 linear: no workspace");
         const dim3 grid((chunks * 8 + 255) / 256, M);
         const cudaError_t err = dtype == QS_F32
@@ -381,6 +397,9 @@ QS_API int qs_q4_linear(void* out, int out_dtype, long long ldo, const void* x, 
         p.x = (const __nv_bfloat16*)scratch;
         p.ldx = (size_t)chunks * 64;
     }
+    if (dtype == QS_BF16 && M >= MANY_ROWS)
+        return q4_linear_many(out, out_dtype, ldo, p.x, (long long)p.ldx, codes, scales, bias, bias_dtype, act, res0, res1, ldr, M, N, chunks, group, settled,
+                              (char*)scratch + rows, status, stream);
     if (group == 32) return few<32>(p, stream);
     if (group == 64) return few<64>(p, stream);
     return few<128>(p, stream);

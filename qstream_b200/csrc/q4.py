@@ -7,27 +7,30 @@ order of the codes here is the one in which the tensor cores take them.
 """
 from __future__ import annotations
 
+import functools
 from ctypes import c_int, c_longlong, c_void_p
 from dataclasses import dataclass
 
 import torch
 
 from ..errors import QsError, QStreamError
-from . import ops
+from . import gemm_tc, ops
 
 GROUPS = (32, 64, 128)
 TYPES = (torch.float32, torch.bfloat16)
 MAX_COLUMNS = 32768
 
-_quantize = _linear = None
+_quantize = _linear = _scratch = _kernels = None
 
 
 def _bind():
-    global _quantize, _linear
+    global _quantize, _linear, _scratch, _kernels
     if _linear is None:
         _quantize = ops.bind("qs_q4_quantize", [c_void_p, c_void_p, c_void_p, c_int, c_longlong, c_int, c_int, c_int, c_void_p])
+        _scratch = functools.lru_cache(maxsize=4096)(ops.bind("qs_q4_linear_scratch", [c_int, c_int, c_int, c_int, c_int], c_longlong))
+        _kernels = functools.lru_cache(maxsize=4096)(ops.bind("qs_q4_linear_kernels", [c_int, c_int, c_int, c_int], c_int))
         _linear = ops.bind("qs_q4_linear", [c_void_p, c_int, c_longlong, c_void_p, c_int, c_longlong, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int,
-                                            c_void_p, c_void_p, c_longlong, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p])
+                                            c_void_p, c_void_p, c_longlong, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p])
 
 
 def _refuse(text, code=QsError.INVALID_INPUT):
@@ -137,11 +140,12 @@ def linear(x, weight: Weight4, bias=None, activation=None, residuals=(), out_dty
     _bind()
     code, element = ops.dtype_code(x), x.element_size()
     aligned = x.data_ptr() % 16 == 0 and ldx * element % 16 == 0
-    scratch = None
-    if code == ops.F32 or K % 64 or not aligned:        # rows laid out anew: whole chunks of 64 columns, three terms to a float32 number
-        scratch = torch.empty((M * (3 if code == ops.F32 else 1), -(-K // 64) * 64), dtype=torch.bfloat16, device=x.device)
-        ops.count_launches(1)
+    nbytes = _scratch(M, N, K, code, int(aligned))          # rows laid out anew, for many rows the operands' powers of two
+    scratch = torch.empty((nbytes,), dtype=torch.uint8, device=x.device) if nbytes else None
+    if nbytes:
+        ops.count_launches(_kernels(M, K, code, int(aligned)) - 1)
     ops.check(_linear(ops.ptr(out), ops.dtype_code(out), out.stride(0), ops.ptr(x), code, ldx, int(aligned), ops.ptr(weight.codes), ops.ptr(weight.scales),
                       ops.ptr(bias), ops.dtype_code(bias) if bias is not None else 0, ops.ACTIVATIONS[activation], ops.ptr(res[0]), ops.ptr(res[1]), ldr,
-                      M, N, K, weight.group, int(bool(settled)), ops.ptr(scratch), ops.stream()))
+                      M, N, K, weight.group, int(bool(settled)), ops.ptr(scratch),
+                      ops.ptr(gemm_tc.status_word(x.device)), ops.stream()))
     return out
