@@ -10,12 +10,13 @@
 //
 // A block takes 128 rows of the matrix and up to 128 rows of x.  Chunk by chunk of 64 columns:
 //   warp 18         copies the codes to shared memory, four chunks of eight tiles at a time (bulk copies)
-//   warps 2 .. 9    take 16 rows each: a code c, shifted into the lowest bits of a 16-bit 1024, is 1024 + c; 1032 less, times the scale; a word of
-//                   eight codes is one chunk of 16 bytes of a row in the layout of the 128-byte swizzle.  Lanes of odd rows write the two halves of the
-//                   columns in the other order, so that two rows' chunks meet all banks
+//   warps 2 .. 17   four teams, a chunk to each; a warp takes 32 rows: a code c, shifted into the lowest bits of a 16-bit 1024, is 1024 + c; 1032 less,
+//                   times the scale; a word of eight codes is one chunk of 16 bytes of a row in the layout of the 128-byte swizzle.  Lanes of
+//                   odd rows write the two halves of the columns in the other order, so that two rows' chunks meet all banks.  (A warp's chunk takes
+//                   1,000 cycles, most of them waits; one team of eight warps: 700 rows, 8,192 x 2,048 were half as fast)
 //   warp 0          copies the rows of x (TMA)
 //   warp 1          multiplies (tcgen05.mma, D [128 x rows of x], 32-bit, in TMEM)
-//   warps 10 .. 17  read D back, and finish
+// In the end D goes through shared memory, so that a warp finishes whole rows of results.
 // Bound by shared memory: a chunk is 16 KB written and read for each operand, 512 cycles where the product takes 256.
 //
 // Where blocks are few, those of a cluster share the columns, and add their sums through distributed shared memory, in their order.
@@ -30,8 +31,8 @@ using namespace sm100;
 
 namespace {
 
-constexpr int BM = 128, BN = 128, KC = 64, STAGES = 4, SLOTS = 3, SLOT_CHUNKS = 4;
-constexpr int DECODERS = 8, FINISHERS = 8, THREADS = (3 + DECODERS + FINISHERS) * 32;
+constexpr int BM = 128, BN = 128, KC = 64, STAGES = 5, SLOTS = 3, SLOT_CHUNKS = 4;
+constexpr int TEAMS = SLOT_CHUNKS, TEAM = 4, DECODERS = TEAMS * TEAM, THREADS = (3 + DECODERS) * 32;
 constexpr int A_BYTES = BM * KC * 2, B_BYTES = BN * KC * 2, SLOT_BYTES = 8 * SLOT_CHUNKS * 512, SMEM = STAGES * (A_BYTES + B_BYTES) + SLOTS * SLOT_BYTES + 1024;
 constexpr int PITCH = BM + 4;                            // of a row of x's sums, floats
 
@@ -42,9 +43,12 @@ struct Many {
     const uint4* codes;
     const uint32_t* scales;
     size_t ldo, ldr;
-    int M, N, chunks, share, columns, out_dtype, bias_dtype, act, settled;
+    int M, N, chunks, share, columns, out_dtype, bias_dtype, act, settled, vector;       // vector: rows of results and residuals on boundaries of four elements
     int32_t* status;
 };
+
+// Not inlined: sixteen copies of every activation are more code than a block runs through, and their way to the SM was a third of the kernel's time.
+__device__ __noinline__ float activated(float v, int act) { return apply_activation_wide(v, act); }
 
 // Columns 2 i, 2 i + 1 of a word's eight, times the scale.
 __device__ __forceinline__ uint32_t two_weights(uint32_t word, int i, uint32_t scale) {
@@ -138,7 +142,7 @@ q4_many_kernel(const __grid_constant__ CUtensorMap map_x, const Many p) {
     const int c0 = (int)rank * p.share, n = max(0, min(p.share, p.chunks - c0));        // this block's chunks
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < STAGES; ++i) { mbar_init(&a_full[i], DECODERS * 32); mbar_init(&b_full[i], 1); mbar_init(&empty[i], 1); }
+        for (int i = 0; i < STAGES; ++i) { mbar_init(&a_full[i], TEAM * 32); mbar_init(&b_full[i], 1); mbar_init(&empty[i], 1); }
         for (int i = 0; i < SLOTS; ++i) { mbar_init(&c_full[i], 1); mbar_init(&c_empty[i], DECODERS); }
         mbar_init(&done, 1);
         aborted = 0;
@@ -186,60 +190,66 @@ q4_many_kernel(const __grid_constant__ CUtensorMap map_x, const Many p) {
         __syncwarp();
     } else if (warp < 2 + DECODERS) {
         // ------------------------------------------------------------------ codes to numbers
-        const int mine = warp - 2, g = lane >> 2, t = lane & 3, odd = g & 1;
+        const int team = (warp - 2) / TEAM, mine = (warp - 2) % TEAM * 2, g = lane >> 2, t = lane & 3, odd = g & 1;      // chunks team, + TEAMS, ..., tiles mine and the next
         bool ok = true;
         grid_dep_wait();
-        // the scales of rows g and g + 8 (both halves of a word), over the rows' powers of two; those of eight groups ahead
-        const size_t tile_at = min((row0 >> 4) + mine, tiles - 1);
-        const uint32_t* scales = p.scales + tile_at * groups * 8 + g;
-        const float inv0 = inverse_of(p.row_unit[tile_at * 16 + g]), inv1 = inverse_of(p.row_unit[tile_at * 16 + 8 + g]);
-        constexpr int PER = GROUP == 32 ? 2 : 1, HALF = 4;                     // groups of a chunk; chunks whose scales are fetched together
-        uint32_t ahead[2][HALF][PER];
-        auto fetch = [&](uint32_t (&to)[HALF][PER], int i) {
+        // the scales of rows g and g + 8 (both halves of a word), over the rows' powers of two; those of two chunks ahead
+        constexpr int PER = GROUP == 32 ? 2 : 1;         // groups of a chunk
+        const uint32_t* scales[2];
+        float inv[2][2];
 #pragma unroll
-            for (int u = 0; u < HALF; ++u)
+        for (int q = 0; q < 2; ++q) {
+            const size_t tile = min((row0 >> 4) + mine + q, tiles - 1);
+            scales[q] = p.scales + tile * groups * 8 + g;
+            inv[q][0] = inverse_of(p.row_unit[tile * 16 + g]);
+            inv[q][1] = inverse_of(p.row_unit[tile * 16 + 8 + g]);
+        }
+        uint32_t ahead[2][PER][2];
+        auto fetch = [&](uint32_t (&to)[PER][2], int i) {
 #pragma unroll
-                for (int h = 0; h < PER; ++h) to[u][h] = __ldg(scales + (size_t)min((c0 + i + u) * 64 / GROUP + h, groups - 1) * 8);
+            for (int h = 0; h < PER; ++h)
+#pragma unroll
+                for (int q = 0; q < 2; ++q) to[h][q] = __ldg(scales[q] + (size_t)min((c0 + i) * 64 / GROUP + h, groups - 1) * 8);
         };
-        fetch(ahead[0], 0);
-        fetch(ahead[1], HALF);
-        for (int i0 = 0; i0 < n && ok; i0 += 2 * HALF)
+        fetch(ahead[0], team);
+        fetch(ahead[1], team + TEAMS);
+        for (int i0 = team; i0 < n && ok; i0 += 2 * TEAMS)
 #pragma unroll
-        for (int ii = 0; ii < 2 * HALF; ++ii) {
-            const int i = i0 + ii;
+        for (int turn = 0; turn < 2; ++turn) {
+            const int i = i0 + turn * TEAMS;
             if (i >= n) break;
-            uint32_t unit[PER][2];
-#pragma unroll
-            for (int h = 0; h < PER; ++h) {
-                const uint32_t pair = ahead[ii / HALF][ii % HALF][h];
-                const __half2 a = __float2half2_rn(__uint_as_float(pair << 16) * inv0), b = __float2half2_rn(__uint_as_float(pair & 0xffff0000u) * inv1);
-                unit[h][0] = *reinterpret_cast<const uint32_t*>(&a);
-                unit[h][1] = *reinterpret_cast<const uint32_t*>(&b);
-            }
-            if (ii == HALF - 1) fetch(ahead[0], i0 + 2 * HALF);
-            if (ii == 2 * HALF - 1) fetch(ahead[1], i0 + 3 * HALF);
             const int st = i % STAGES, slot = i / SLOT_CHUNKS % SLOTS;
-            if (i % SLOT_CHUNKS == 0 && !mbar_wait(&c_full[slot], (i / SLOT_CHUNKS / SLOTS) & 1)) ok = false;
+            if (!mbar_wait(&c_full[slot], (i / SLOT_CHUNKS / SLOTS) & 1)) ok = false;
             if (ok && (aborted || !mbar_wait(&empty[st], ((i / STAGES) & 1) ^ 1))) ok = false;
             if (!ok) { if (lane == 0) atomicExch(p.status, 133); aborted = 1; break; }
-            const uint4 raw = *reinterpret_cast<const uint4*>(slots + slot * SLOT_BYTES + (mine * SLOT_CHUNKS + i % SLOT_CHUNKS) * 512 + lane * 16);
-            uint8_t* tile = smem + st * (A_BYTES + B_BYTES) + (16 * mine + g) * 128;
-            // words: row g and g + 8, columns 0 .. 31, then the same of 32 .. 63; odd rows the other way round
-            const uint32_t w[4] = {odd ? raw.z : raw.x, odd ? raw.w : raw.y, odd ? raw.x : raw.z, odd ? raw.y : raw.w};
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int at = ((4 * ((k >> 1) ^ odd) + t) ^ g) << 4;
-                const uint32_t s = PER == 1 ? unit[0][k & 1] : (k >> 1) ^ odd ? unit[PER - 1][k & 1] : unit[0][k & 1];
-                *reinterpret_cast<uint4*>(tile + (k & 1) * 8 * 128 + at) = make_uint4(two_weights(w[k], 0, s), two_weights(w[k], 1, s), two_weights(w[k], 2, s), two_weights(w[k], 3, s));
+            for (int q = 0; q < 2; ++q) {
+                uint32_t unit[PER][2];
+#pragma unroll
+                for (int h = 0; h < PER; ++h) {
+                    const uint32_t pair = ahead[turn][h][q];
+                    const __half2 a = __float2half2_rn(__uint_as_float(pair << 16) * inv[q][0]), b = __float2half2_rn(__uint_as_float(pair & 0xffff0000u) * inv[q][1]);
+                    unit[h][0] = *reinterpret_cast<const uint32_t*>(&a);
+                    unit[h][1] = *reinterpret_cast<const uint32_t*>(&b);
+                }
+                const uint4 raw = *reinterpret_cast<const uint4*>(slots + slot * SLOT_BYTES + ((mine + q) * SLOT_CHUNKS + i % SLOT_CHUNKS) * 512 + lane * 16);
+                uint8_t* tile = smem + st * (A_BYTES + B_BYTES) + (16 * (mine + q) + g) * 128;
+                // words: row g and g + 8, columns 0 .. 31, then the same of 32 .. 63; odd rows the other way round
+                const uint32_t w[4] = {odd ? raw.z : raw.x, odd ? raw.w : raw.y, odd ? raw.x : raw.z, odd ? raw.y : raw.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int at = ((4 * ((k >> 1) ^ odd) + t) ^ g) << 4;
+                    const uint32_t s = PER == 1 ? unit[0][k & 1] : (k >> 1) ^ odd ? unit[PER - 1][k & 1] : unit[0][k & 1];
+                    *reinterpret_cast<uint4*>(tile + (k & 1) * 8 * 128 + at) = make_uint4(two_weights(w[k], 0, s), two_weights(w[k], 1, s), two_weights(w[k], 2, s), two_weights(w[k], 3, s));
+                }
             }
             fence_proxy_async_smem();
             mbar_arrive(&a_full[st]);
-            if (i % SLOT_CHUNKS == SLOT_CHUNKS - 1) {
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&c_empty[slot]);
-            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&c_empty[slot]);
+            fetch(ahead[turn], i + 2 * TEAMS);
         }
-    } else if (warp == 2 + DECODERS + FINISHERS) {
+    } else {
         // ------------------------------------------------------------------ codes
         if (!p.settled) grid_dep_wait();
         if (elect_one()) {
@@ -259,57 +269,90 @@ q4_many_kernel(const __grid_constant__ CUtensorMap map_x, const Many p) {
         }
         __syncwarp();
         if (p.settled) grid_dep_wait();
-    } else {
-        // ------------------------------------------------------------------ results
-        grid_dep_wait();
-        if (!mbar_wait(&done, 0)) { if (lane == 0) atomicExch(p.status, 134); aborted = 1; }
-        tc_fence_after_sync();
     }
+    __syncwarp();
     grid_dep_launch();
 
-    auto finish = [&](float y, int row, int m) {
-        y = y * p.row_unit[row] * p.x_unit[m];
-        if (p.bias) y += load_as_f32(p.bias, p.bias_dtype, row);
-        if (p.act != QS_ACT_NONE) y = apply_activation_wide(y, p.act);
-        if (p.res0) y += load_as_f32(p.res0, QS_BF16, (size_t)m * p.ldr + row);
-        if (p.res1) y += load_as_f32(p.res1, QS_BF16, (size_t)m * p.ldr + row);
-        store_from_f32(p.out, p.out_dtype, (size_t)m * p.ldo + row, y);
-    };
-    float* part = reinterpret_cast<float*>(smem);        // [row of x][row of the matrix]; the stages are free
-    if (warp >= 2 + DECODERS && warp < 2 + DECODERS + FINISHERS) {
-        const int r = (warp & 3) * 32 + lane, half = (warp - 2 - DECODERS) >> 2;
+    // ------------------------------------------------------------------ results
+    if (!mbar_wait(&done, 0)) { if (lane == 0) atomicExch(p.status, 134); aborted = 1; }
+    __syncthreads();                                     // nobody waits for a copy or reads a stage any more
+    tc_fence_after_sync();
+    float* part = reinterpret_cast<float*>(smem);        // [row of x][row of the matrix], where the stages were
+    if (warp >= 4 && warp < 12) {                        // a warp may read the lanes 32 (warp % 4) ...: two warps to each 32 rows of the matrix
+        const int r = (warp & 3) * 32 + lane, half = (warp - 4) >> 2;
         for (int q = half * 64; q < min(half * 64 + 64, p.columns); q += 16) {
             uint32_t d[16];
             tmem_load_32x16(tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)q, d);
             tmem_load_wait();
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const float y = n > 0 ? __uint_as_float(d[j]) : 0.f;
-                if (blocks > 1) part[(q + j) * PITCH + r] = y;
-                else if (!aborted && row0 + r < p.N && m0 + q + j < p.M) finish(y, row0 + r, m0 + q + j);
-            }
+            for (int j = 0; j < 16; ++j) part[(q + j) * PITCH + r] = n > 0 ? __uint_as_float(d[j]) : 0.f;
         }
     }
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
     if (warp == 1) tmem_dealloc(tmem, BN);
-    if (blocks > 1) {
-        cluster_sync();
-        const int rows = min(p.columns, p.M - m0);
-        for (int i = threadIdx.x + rank * THREADS; i < rows * BM; i += blocks * THREADS) {
-            const int j = i / BM, rr = i % BM;
-            if (row0 + rr >= p.N) continue;
-            float y = 0.f;
-            for (uint32_t b = 0; b < blocks; ++b) {
-                float v;
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_cta(part + j * PITCH + rr, b)) : "memory");
-                y += v;
-            }
-            if (!aborted) finish(y, row0 + rr, m0 + j);
-        }
-        cluster_sync();                                  // the others have read this block's sums
+    if (blocks > 1) cluster_sync();
+    // a warp takes a row of x, a lane four rows of the matrix
+    const int row = row0 + 4 * lane, here = max(0, min(4, p.N - row));
+    float row_unit[4], bias[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        row_unit[k] = k < here ? p.row_unit[row + k] : 0.f;
+        bias[k] = p.bias && k < here ? load_as_f32(p.bias, p.bias_dtype, row + k) : 0.f;
     }
+    if (!aborted)
+        for (int j = warp * blocks + rank; j < min(p.columns, p.M - m0); j += THREADS / 32 * blocks) {
+            const size_t m = m0 + j;
+            const float unit = p.x_unit[m];
+            float y[4] = {0.f, 0.f, 0.f, 0.f};
+            if (blocks == 1) {
+                const float4 v = *reinterpret_cast<const float4*>(part + j * PITCH + 4 * lane);
+                y[0] = v.x; y[1] = v.y; y[2] = v.z; y[3] = v.w;
+            } else {
+                for (uint32_t b = 0; b < blocks; ++b) {
+                    float v[4];
+                    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(map_to_cta(part + j * PITCH + 4 * lane, b)) : "memory");
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) y[k] += v[k];
+                }
+            }
+            float add[4] = {0.f, 0.f, 0.f, 0.f};
+            const __nv_bfloat16* res[2] = {reinterpret_cast<const __nv_bfloat16*>(p.res0), reinterpret_cast<const __nv_bfloat16*>(p.res1)};
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (res[i]) {
+                    const __nv_bfloat16* src = res[i] + m * p.ldr + row;
+                    if (here == 4 && p.vector) {
+                        const uint2 raw = *reinterpret_cast<const uint2*>(src);
+                        add[0] += __uint_as_float(raw.x << 16); add[1] += __uint_as_float(raw.x & 0xffff0000u);
+                        add[2] += __uint_as_float(raw.y << 16); add[3] += __uint_as_float(raw.y & 0xffff0000u);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (k < here) add[k] += to_f32(src[k]);
+                    }
+                }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                y[k] = y[k] * row_unit[k] * unit + bias[k];
+                if (p.act != QS_ACT_NONE) y[k] = activated(y[k], p.act);
+                y[k] += add[k];
+            }
+            if (here == 4 && p.vector) {
+                if (p.out_dtype == QS_F32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + m * p.ldo + row) = make_float4(y[0], y[1], y[2], y[3]);
+                else {
+                    const __nv_bfloat162 a = __floats2bfloat162_rn(y[0], y[1]), b = __floats2bfloat162_rn(y[2], y[3]);
+                    *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(p.out) + m * p.ldo + row) =
+                        make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (k < here) store_from_f32(p.out, p.out_dtype, m * p.ldo + row + k, y[k]);
+            }
+        }
+    if (blocks > 1) cluster_sync();                      // the others have read this block's sums
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
@@ -381,8 +424,10 @@ int q4_linear_many(void* out, int out_dtype, long long ldo, const void* x, long 
     const CUresult rc = fn(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, xh, dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (rc != CUDA_SUCCESS) return qs_fail(QS_ERR_INTERNAL, "q4 linear: cuTensorMapEncodeTiled failed with %d", (int)rc);
+    const int o = out_dtype == QS_F32 ? 16 : 8;
+    const int vector = ((uintptr_t)out % o) == 0 && ldo % 4 == 0 && ldr % 4 == 0 && ((uintptr_t)res0 % 8) == 0 && ((uintptr_t)res1 % 8) == 0;
     const Many p = {out, row_unit, x_unit, bias, res0, res1, (const uint4*)codes, (const uint32_t*)scales, (size_t)ldo, (size_t)ldr, M, N, chunks, (chunks + blocks - 1) / blocks, columns,
-                    out_dtype, bias_dtype, act, settled, status};
+                    out_dtype, bias_dtype, act, settled, vector, status};
     const dim3 grid(row_tiles * blocks, column_tiles);
     if (group == 32) return go<32>(p, map, grid, blocks, stream);
     if (group == 64) return go<64>(p, map, grid, blocks, stream);
