@@ -18,8 +18,10 @@ long long q4_many_scratch(int M, int N, int chunks);
 
 namespace {
 
-// From how many bfloat16 rows on the products go to the 5th-generation tensor cores.
-constexpr int MANY_ROWS = 17;
+// Which bfloat16 products go to the 5th-generation tensor cores: those of more than 16 rows that are large enough for what they take beside (some 12 us for the
+// powers of two, the way of the first chunk and of the results).  Microseconds, 16 rows at a time here | there: 32 rows, 2,048 x 2,048: 7 | 17, 4,096 x 4,096:
+// 13 | 16, 16,384 x 4,096: 42 | 36, 4,096 x 16,384: 53 | 39; 64 rows: 12 | 19, 27 | 17, 84 | 37, 101 | 41.
+bool many_rows(int M, int N, int K, int dtype) { return dtype == QS_BF16 && M > 16 && (double)M * N * K >= 6e8; }
 
 // The column within eight of a word's i-th code.
 __device__ __forceinline__ int column_of(int i) { return i < 4 ? 2 * i : 2 * i - 7; }
@@ -366,9 +368,9 @@ static long long rows_scratch(int M, int K, int dtype, int aligned) {
 
 // Bytes of workspace that `qs_q4_linear` takes, and its kernels.
 QS_API long long qs_q4_linear_scratch(int M, int N, int K, int dtype, int aligned) {
-    return rows_scratch(M, K, dtype, aligned) + (dtype == QS_BF16 && M >= MANY_ROWS ? q4_many_scratch(M, N, (K + 63) / 64) : 0);
+    return rows_scratch(M, K, dtype, aligned) + (many_rows(M, N, K, dtype) ? q4_many_scratch(M, N, (K + 63) / 64) : 0);
 }
-QS_API int qs_q4_linear_kernels(int M, int K, int dtype, int aligned) { return 1 + (rows_scratch(M, K, dtype, aligned) > 0) + (dtype == QS_BF16 && M >= MANY_ROWS); }
+QS_API int qs_q4_linear_kernels(int M, int N, int K, int dtype, int aligned) { return 1 + (rows_scratch(M, K, dtype, aligned) > 0) + many_rows(M, N, K, dtype); }
 
 // out [M, N] = act(x W^T + bias) + residuals; x of type `dtype`, out of type `out_dtype` (float32 for float32 rows).  `aligned`: rows of x begin on
 // 16-byte boundaries.  `settled`: codes and scales were complete before the previous kernel of the stream began; the kernel then reads them while that kernel
@@ -397,7 +399,7 @@ QS_API int qs_q4_linear(void* out, int out_dtype, long long ldo, const void* x, 
         p.x = (const __nv_bfloat16*)scratch;
         p.ldx = (size_t)chunks * 64;
     }
-    if (dtype == QS_BF16 && M >= MANY_ROWS)
+    if (many_rows(M, N, K, dtype))
         return q4_linear_many(out, out_dtype, ldo, p.x, (long long)p.ldx, codes, scales, bias, bias_dtype, act, res0, res1, ldr, M, N, chunks, group, settled,
                               (char*)scratch + rows, status, stream);
     if (group == 32) return few<32>(p, stream);

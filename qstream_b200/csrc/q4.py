@@ -28,7 +28,7 @@ def _bind():
     if _linear is None:
         _quantize = ops.bind("qs_q4_quantize", [c_void_p, c_void_p, c_void_p, c_int, c_longlong, c_int, c_int, c_int, c_void_p])
         _scratch = functools.lru_cache(maxsize=4096)(ops.bind("qs_q4_linear_scratch", [c_int, c_int, c_int, c_int, c_int], c_longlong))
-        _kernels = functools.lru_cache(maxsize=4096)(ops.bind("qs_q4_linear_kernels", [c_int, c_int, c_int, c_int], c_int))
+        _kernels = functools.lru_cache(maxsize=4096)(ops.bind("qs_q4_linear_kernels", [c_int, c_int, c_int, c_int, c_int], c_int))
         _linear = ops.bind("qs_q4_linear", [c_void_p, c_int, c_longlong, c_void_p, c_int, c_longlong, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int,
                                             c_void_p, c_void_p, c_longlong, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p])
 
@@ -143,7 +143,7 @@ def linear(x, weight: Weight4, bias=None, activation=None, residuals=(), out_dty
     nbytes = _scratch(M, N, K, code, int(aligned))          # rows laid out anew, for many rows the operands' powers of two
     scratch = torch.empty((nbytes,), dtype=torch.uint8, device=x.device) if nbytes else None
     if nbytes:
-        ops.count_launches(_kernels(M, K, code, int(aligned)) - 1)
+        ops.count_launches(_kernels(M, N, K, code, int(aligned)) - 1)
     ops.check(_linear(ops.ptr(out), ops.dtype_code(out), out.stride(0), ops.ptr(x), code, ldx, int(aligned), ops.ptr(weight.codes), ops.ptr(weight.scales),
                       ops.ptr(bias), ops.dtype_code(bias) if bias is not None else 0, ops.ACTIVATIONS[activation], ops.ptr(res[0]), ops.ptr(res[1]), ldr,
                       M, N, K, weight.group, int(bool(settled)), ops.ptr(scratch),

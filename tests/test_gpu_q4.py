@@ -171,3 +171,34 @@ def test_many_columns(n, k):
             x = normal(m, m, k, dtype=dtype)
             want, bound = U.linear(U.f64(x), U.dense(w), out_bf16=dtype == torch.bfloat16)
             assert (np.abs(U.f64(q4.linear(x, w)) - want) <= bound).all(), m
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("m,n,k", [(17, 6000, 6016), (130, 2100, 2500), (300, 1000, 2048), (33, 1100, 17000), (1000, 130, 4800), (3000, 16, 12800)])
+def test_products_of_many_rows(m, n, k, group):
+    """Those that the 5th-generation tensor cores take, with ragged rows, columns and tiles, and what comes behind them."""
+    w = q4.quantize(normal(n + k, n, k, std=0.05), group)
+    dense = U.dense(w)
+    wide = normal(m, m, k + 8, dtype=torch.bfloat16)
+    bias, r0, r1 = normal(3, n), normal(4, m, n, dtype=torch.bfloat16), normal(5, m, n, dtype=torch.bfloat16)
+    for at in (0, 8, 3):                                    # rows on 16-byte boundaries and off them
+        x = wide[:, at:at + k] if at + k <= k + 8 else wide
+        for args, kw in (((), {}), ((bias, "gelu_new", (r0, r1)), {}), ((bias, None, (r0,), torch.float32), {})):
+            res = [U.f64(r) for r in args[2]] if len(args) > 2 else []
+            want, bound = U.linear(U.f64(x), dense, U.f64(bias) if args else None, args[1] if args else None, res, out_bf16=len(args) < 4)
+            got = U.f64(q4.linear(x, w, *args))
+            assert (np.abs(got - want) <= bound).all(), (at, len(args), (np.abs(got - want) / bound).max())
+    out = torch.full((m, n + 7), 7.0, dtype=torch.bfloat16, device="cuda")
+    q4.linear(x, w, out=out[:, 3:3 + n])
+    want, bound = U.linear(U.f64(x), dense, out_bf16=True)
+    assert (np.abs(U.f64(out[:, 3:3 + n]) - want) <= bound).all() and (out[:, :3] == 7).all() and (out[:, 3 + n:] == 7).all()
+    y = x.clone()
+    y[0, 7], y[-1, 0] = float("nan"), float("inf")
+    got = q4.linear(y, w)
+    plain = q4.linear(x, w)
+    assert not torch.isfinite(got[0]).any() and not torch.isfinite(got[-1]).all() and torch.equal(got[1:-1], plain[1:-1])
+    # rows and scales of very different sizes keep their own precision
+    z = x * torch.logspace(-30, 30, m, device="cuda")[:, None].bfloat16()
+    big = q4.Weight4(w.codes, w.scales * torch.logspace(-2, 2, w.scales.shape[0], device="cuda")[:, None, None, None].bfloat16(), n, k, group)
+    want, bound = U.linear(U.f64(z), U.dense(big), out_bf16=True)
+    assert (np.abs(U.f64(q4.linear(z, big)) - want) <= bound).all()
