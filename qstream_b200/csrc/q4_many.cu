@@ -31,9 +31,9 @@ using namespace sm100;
 
 namespace {
 
-constexpr int BM = 128, BN = 128, KC = 64, STAGES = 5, SLOTS = 3, SLOT_CHUNKS = 4;
+constexpr int BM = 128, BN = 128, KC = 64, STAGES = 3, SLOTS = 2, SLOT_CHUNKS = 4;        // a stage holds two chunks
 constexpr int TEAMS = SLOT_CHUNKS, TEAM = 4, DECODERS = TEAMS * TEAM, THREADS = (3 + DECODERS) * 32;
-constexpr int A_BYTES = BM * KC * 2, B_BYTES = BN * KC * 2, SLOT_BYTES = 8 * SLOT_CHUNKS * 512, SMEM = STAGES * (A_BYTES + B_BYTES) + SLOTS * SLOT_BYTES + 1024;
+constexpr int A_BYTES = BM * KC * 2, B_BYTES = BN * KC * 2, SLOT_BYTES = 8 * SLOT_CHUNKS * 512, STAGE_BYTES = 2 * (A_BYTES + B_BYTES), SMEM = STAGES * STAGE_BYTES + SLOTS * SLOT_BYTES + 1024;
 constexpr int PITCH = BM + 4;                            // of a row of x's sums, floats
 
 struct Many {
@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 q4_many_kernel(const __grid_constant__ CUtensorMap map_x, const Many p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    __shared__ uint64_t a_full[STAGES], b_full[STAGES], empty[STAGES], done, c_full[SLOTS], c_empty[SLOTS];
+    __shared__ uint64_t full[STAGES], empty[STAGES], done, c_full[SLOTS], c_empty[SLOTS];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int aborted;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -142,7 +142,7 @@ q4_many_kernel(const __grid_constant__ CUtensorMap map_x, const Many p) {
     const int c0 = (int)rank * p.share, n = max(0, min(p.share, p.chunks - c0));        // this block's chunks
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < STAGES; ++i) { mbar_init(&a_full[i], TEAM * 32); mbar_init(&b_full[i], 1); mbar_init(&empty[i], 1); }
+        for (int i = 0; i < STAGES; ++i) { mbar_init(&full[i], 2 * TEAM * 32 + 1); mbar_init(&empty[i], 1); }
         for (int i = 0; i < SLOTS; ++i) { mbar_init(&c_full[i], 1); mbar_init(&c_empty[i], DECODERS); }
         mbar_init(&done, 1);
         aborted = 0;
@@ -154,20 +154,23 @@ q4_many_kernel(const __grid_constant__ CUtensorMap map_x, const Many p) {
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = tmem_slot;
-    uint8_t* slots = smem + STAGES * (A_BYTES + B_BYTES);
+    uint8_t* slots = smem + STAGES * STAGE_BYTES;
+    const int pairs = (n + 1) >> 1;
 
     if (warp == 0) {
         // ------------------------------------------------------------------ rows of x
         grid_dep_wait();
         if (elect_one()) {
             int i = 0;
-            for (; i < n && !aborted; ++i) {
-                const int st = i % STAGES;
+            for (; i < pairs && !aborted; ++i) {
+                const int st = i % STAGES, here = min(2, n - 2 * i);
                 if (!mbar_wait(&empty[st], ((i / STAGES) & 1) ^ 1)) { atomicExch(p.status, 130); aborted = 1; break; }
-                mbar_expect_tx(&b_full[st], p.columns * KC * 2);
-                tma_load_2d(smem + st * (A_BYTES + B_BYTES) + A_BYTES, &map_x, &b_full[st], (c0 + i) * KC, m0);
+                uint8_t* dst = smem + st * STAGE_BYTES + 2 * A_BYTES;
+                mbar_expect_tx(&full[st], here * p.columns * KC * 2);
+                for (int k = 0; k < here; ++k) tma_load_2d(dst + k * B_BYTES, &map_x, &full[st], (c0 + 2 * i + k) * KC, m0);
             }
-            for (int k = max(0, i - STAGES); k < i; ++k) mbar_wait(&b_full[k % STAGES], (k / STAGES) & 1);       // no copy outlives the block
+            if (aborted)                                 // no copy outlives the block (the other arrivals of the phase may be missing: until the limit)
+                for (int k = max(0, i - STAGES); k < i; ++k) mbar_wait(&full[k % STAGES], (k / STAGES) & 1);
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -175,13 +178,15 @@ q4_many_kernel(const __grid_constant__ CUtensorMap map_x, const Many p) {
         grid_dep_wait();
         if (elect_one()) {
             const uint32_t idesc = idesc_of(p.columns);
-            for (int i = 0; i < n && !aborted; ++i) {
-                const int st = i % STAGES;
-                if (!mbar_wait(&a_full[st], (i / STAGES) & 1) || !mbar_wait(&b_full[st], (i / STAGES) & 1)) { atomicExch(p.status, 131); aborted = 1; break; }
+            for (int i = 0; i < pairs && !aborted; ++i) {
+                const int st = i % STAGES, steps = min(8, 4 * (n - 2 * i));
+                if (!mbar_wait(&full[st], (i / STAGES) & 1)) { atomicExch(p.status, 131); aborted = 1; break; }
                 tc_fence_after_sync();
-                const uint32_t a = smem_u32(smem + st * (A_BYTES + B_BYTES)), b = a + A_BYTES;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) mma_bf16(tmem, smem_desc_sw128(a + k * 32), smem_desc_sw128(b + k * 32), idesc, (i | k) != 0);
+                const uint32_t a = smem_u32(smem + st * STAGE_BYTES), b = a + 2 * A_BYTES;
+                for (int k = 0; k < steps; ++k) {
+                    const uint32_t at = (k >> 2) * A_BYTES + (k & 3) * 32;     // (a chunk of the rows of x takes as much)
+                    mma_bf16(tmem, smem_desc_sw128(a + at), smem_desc_sw128(b + at), idesc, (i | k) != 0);
+                }
                 mma_commit(&empty[st]);
             }
             mma_commit(&done);                           // nor a product
@@ -213,27 +218,28 @@ q4_many_kernel(const __grid_constant__ CUtensorMap map_x, const Many p) {
         };
         fetch(ahead[0], team);
         fetch(ahead[1], team + TEAMS);
-        for (int i0 = team; i0 < n && ok; i0 += 2 * TEAMS)
+        for (int i0 = team; i0 < 2 * pairs && ok; i0 += 2 * TEAMS)
 #pragma unroll
         for (int turn = 0; turn < 2; ++turn) {
             const int i = i0 + turn * TEAMS;
-            if (i >= n) break;
-            const int st = i % STAGES, slot = i / SLOT_CHUNKS % SLOTS;
+            if (i >= 2 * pairs) break;
+            const int pair = i >> 1, st = pair % STAGES, slot = i / SLOT_CHUNKS % SLOTS;
+            if (i >= n) { mbar_arrive(&full[st]); break; }     // half a stage at the end: nothing to write
             if (!mbar_wait(&c_full[slot], (i / SLOT_CHUNKS / SLOTS) & 1)) ok = false;
-            if (ok && (aborted || !mbar_wait(&empty[st], ((i / STAGES) & 1) ^ 1))) ok = false;
+            if (ok && (aborted || !mbar_wait(&empty[st], ((pair / STAGES) & 1) ^ 1))) ok = false;
             if (!ok) { if (lane == 0) atomicExch(p.status, 133); aborted = 1; break; }
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
                 uint32_t unit[PER][2];
 #pragma unroll
                 for (int h = 0; h < PER; ++h) {
-                    const uint32_t pair = ahead[turn][h][q];
-                    const __half2 a = __float2half2_rn(__uint_as_float(pair << 16) * inv[q][0]), b = __float2half2_rn(__uint_as_float(pair & 0xffff0000u) * inv[q][1]);
+                    const uint32_t two = ahead[turn][h][q];
+                    const __half2 a = __float2half2_rn(__uint_as_float(two << 16) * inv[q][0]), b = __float2half2_rn(__uint_as_float(two & 0xffff0000u) * inv[q][1]);
                     unit[h][0] = *reinterpret_cast<const uint32_t*>(&a);
                     unit[h][1] = *reinterpret_cast<const uint32_t*>(&b);
                 }
                 const uint4 raw = *reinterpret_cast<const uint4*>(slots + slot * SLOT_BYTES + ((mine + q) * SLOT_CHUNKS + i % SLOT_CHUNKS) * 512 + lane * 16);
-                uint8_t* tile = smem + st * (A_BYTES + B_BYTES) + (16 * (mine + q) + g) * 128;
+                uint8_t* tile = smem + st * STAGE_BYTES + (i & 1) * A_BYTES + (16 * (mine + q) + g) * 128;
                 // words: row g and g + 8, columns 0 .. 31, then the same of 32 .. 63; odd rows the other way round
                 const uint32_t w[4] = {odd ? raw.z : raw.x, odd ? raw.w : raw.y, odd ? raw.x : raw.z, odd ? raw.y : raw.w};
 #pragma unroll
@@ -244,7 +250,7 @@ q4_many_kernel(const __grid_constant__ CUtensorMap map_x, const Many p) {
                 }
             }
             fence_proxy_async_smem();
-            mbar_arrive(&a_full[st]);
+            mbar_arrive(&full[st]);
             __syncwarp();
             if (lane == 0) mbar_arrive(&c_empty[slot]);
             fetch(ahead[turn], i + 2 * TEAMS);
