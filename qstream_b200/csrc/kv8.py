@@ -7,13 +7,13 @@ reads as NaN until it starts afresh.  The reference keeps its cache in 8 bits wi
 """
 from __future__ import annotations
 
+import functools
 from ctypes import c_float, c_int, c_longlong, c_void_p
 
 import torch
 
-from ..errors import QsError, QStreamError
 from . import ops
-from .q4 import TYPES, _on_current_device, _refuse
+from .q4 import TYPES, _refuse, launch_stream
 
 PAGE_TOKENS = 64
 MAX_SPLIT_CONTEXT = 4096 * 128      # what the merge of the keys' parts holds for any head size; longer contexts go a row at a time
@@ -31,7 +31,7 @@ def _bind():
         _decode = ops.bind("qs_kv8_decode", [
             c_void_p, c_int, c_longlong, c_void_p, c_int, c_longlong, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
             c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p, c_float, c_int, c_void_p, c_void_p, c_void_p])
-        _scratch = ops.bind("qs_kv8_decode_scratch", [c_int, c_int, c_int, c_int, c_int], c_longlong)
+        _scratch = functools.lru_cache(maxsize=4096)(ops.bind("qs_kv8_decode_scratch", [c_int, c_int, c_int, c_int, c_int], c_longlong))
         _prefill = ops.bind("qs_kv8_prefill", [
             c_void_p, c_int, c_longlong, c_void_p, c_longlong, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p,
             c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p, c_float, c_void_p, c_void_p])
@@ -41,26 +41,36 @@ def _bind():
             c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p])
 
 
-def _check_cache(what, k_cache, v_cache, k_scale, v_scale, n_kv_heads, head_dim, v_head_dim, page_tokens):
+def _check_cache(what, k_cache, v_cache, k_scale, v_scale, n_kv_heads, head_dim, v_head_dim, page_tokens) -> int:
+    """The number of pages."""
     if page_tokens != PAGE_TOKENS:
         _refuse(f"{what}: pages of {page_tokens} tokens, the kernels are built for {PAGE_TOKENS}")
-    for name, cache, scale, dim in (("k", k_cache, k_scale, head_dim), ("v", v_cache, v_scale, v_head_dim)):
-        if cache.dtype != torch.int8 or cache.dim() != 4 or tuple(cache.shape[1:]) != (n_kv_heads, PAGE_TOKENS, dim) or not cache.is_contiguous() or cache.shape[0] < 1:
-            _refuse(f"{what}: {name}_cache is contiguous int8 [pages, {n_kv_heads}, {PAGE_TOKENS}, {dim}], got {cache.dtype} {tuple(cache.shape)}")
-        if scale.dtype != torch.float32 or tuple(scale.shape) != tuple(cache.shape[:2]) or not scale.is_contiguous():
-            _refuse(f"{what}: {name}_scale is contiguous float32 {tuple(cache.shape[:2])}, got {scale.dtype} {tuple(scale.shape)}")
-    if k_cache.shape[0] != v_cache.shape[0]:
-        _refuse(f"{what}: {k_cache.shape[0]} pages of keys and {v_cache.shape[0]} of values")
+    shape = k_cache.shape
+    n = shape[0] if len(shape) == 4 else 0
+    if (n < 1 or n_kv_heads < 1 or head_dim < 1 or v_head_dim < 1 or shape != (n, n_kv_heads, PAGE_TOKENS, head_dim) or v_cache.shape != (n, n_kv_heads, PAGE_TOKENS, v_head_dim) or k_cache.dtype is not torch.int8
+            or v_cache.dtype is not torch.int8 or not k_cache.is_contiguous() or not v_cache.is_contiguous()):
+        _refuse(f"{what}: caches are contiguous int8 [pages, {n_kv_heads}, {PAGE_TOKENS}, {head_dim} and {v_head_dim}], got {k_cache.dtype} {tuple(shape)} and "
+                f"{v_cache.dtype} {tuple(v_cache.shape)}")
+    pages = (n, n_kv_heads)
+    if (k_scale.shape != pages or v_scale.shape != pages or k_scale.dtype is not torch.float32 or v_scale.dtype is not torch.float32
+            or not k_scale.is_contiguous() or not v_scale.is_contiguous()):
+        _refuse(f"{what}: scales are contiguous float32 {pages}, got {k_scale.dtype} {tuple(k_scale.shape)} and {v_scale.dtype} {tuple(v_scale.shape)}")
+    return n
 
 
 def _check_int32(what, name, t, dims, n=None):
-    if t.dtype != torch.int32 or t.dim() != dims or not t.is_contiguous() or (n is not None and t.shape[0] != n) or (dims == 2 and 0 in t.shape):
-        _refuse(f"{what}: {name} is a contiguous int32 tensor of {dims} dims{'' if n is None else f', {n} rows'}, got {t.dtype} {tuple(t.shape)}")
+    shape = t.shape
+    if t.dtype is not torch.int32 or len(shape) != dims or not t.is_contiguous() or (n is not None and shape[0] != n) or (dims == 2 and 0 in shape):
+        _refuse(f"{what}: {name} is a contiguous int32 tensor of {dims} dims{'' if n is None else f', {n} rows'}, got {t.dtype} {tuple(shape)}")
 
 
 def _check_status(what, status):
-    if status.dtype != torch.int32 or status.numel() < 1:
+    if status.dtype is not torch.int32 or status.numel() < 1:
         _refuse(f"{what}: the status word is int32")
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
 
 
 def rope_store(q, k, v, n_heads, n_kv_heads, head_dim, rotary_dim, cos_sin, tok_slot, tok_pos, page_table, page_tokens, k_cache, v_cache,
@@ -71,7 +81,7 @@ def rope_store(q, k, v, n_heads, n_kv_heads, head_dim, rotary_dim, cos_sin, tok_
     a second run of rows names in the same call gets the first run only, and status 5."""
     what = "kv8.rope_store"
     dv = int(v_head_dim or head_dim)
-    _check_cache(what, k_cache, v_cache, k_scale, v_scale, n_kv_heads, head_dim, dv, page_tokens)
+    n_pages = _check_cache(what, k_cache, v_cache, k_scale, v_scale, n_kv_heads, head_dim, dv, page_tokens)
     T, wk, ldk = ops._rows(k)
     _, wv, ldv = ops._rows(v)
     if k.dtype not in TYPES or v.dtype != k.dtype or v.shape[0] != T or wk != n_kv_heads * head_dim or wv != n_kv_heads * dv:
@@ -96,14 +106,15 @@ def rope_store(q, k, v, n_heads, n_kv_heads, head_dim, rotary_dim, cos_sin, tok_
     _check_status(what, status)
     if T == 0:
         return
-    _on_current_device(k, v, q, q_out, v_first, cos_sin, tok_slot, tok_pos, page_table, k_cache, v_cache, k_scale, v_scale, status)
-    ops.ptr(k)
-    _bind()
-    ops.check(_store(ops.ptr(q_out), q_out.stride(0) if q is not None else 0, ops.ptr(q), q.stride(0) if q is not None else 0, ops.ptr(k), ldk, ops.ptr(v), ldv,
-                     ops.ptr(v_first), v_first.stride(0) if v_first is not None else 0, float(v_mix), ops.dtype_code(k), T, n_heads if q is not None else 0,
-                     n_kv_heads, head_dim, dv, rotary_dim if cos_sin is not None else 0, ops.ptr(cos_sin), cos_sin.shape[0] if cos_sin is not None else 0,
-                     int(bool(half_layout)), ops.ptr(tok_slot), ops.ptr(tok_pos), ops.ptr(page_table), page_table.shape[0], page_table.shape[1],
-                     k_cache.shape[0], ops.ptr(k_cache), ops.ptr(v_cache), ops.ptr(k_scale), ops.ptr(v_scale), ops.ptr(status), ops.stream()))
+    stream = launch_stream(k.get_device(), v, q, q_out, v_first, cos_sin, tok_slot, tok_pos, page_table, k_cache, v_cache, k_scale, v_scale, status)
+    if _store is None:
+        _bind()
+    slots, max_pages = page_table.shape
+    ops.check(_store(_at(q_out), q_out.stride(0) if q is not None else 0, _at(q), q.stride(0) if q is not None else 0, k.data_ptr(), ldk, v.data_ptr(), ldv,
+                     _at(v_first), v_first.stride(0) if v_first is not None else 0, float(v_mix), ops.dtype_code(k), T, n_heads if q is not None else 0,
+                     n_kv_heads, head_dim, dv, rotary_dim if cos_sin is not None else 0, _at(cos_sin), cos_sin.shape[0] if cos_sin is not None else 0,
+                     1 if half_layout else 0, tok_slot.data_ptr(), tok_pos.data_ptr(), page_table.data_ptr(), slots, max_pages, n_pages, k_cache.data_ptr(),
+                     v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), status.data_ptr(), stream))
 
 
 def read_pages(cache, scale, pages, dtype=torch.float32) -> torch.Tensor:
@@ -112,28 +123,31 @@ def read_pages(cache, scale, pages, dtype=torch.float32) -> torch.Tensor:
     what = "kv8.read_pages"
     if cache.dim() != 4 or scale.dim() != 2:
         _refuse(f"{what}: a cache {tuple(cache.shape)} with scales {tuple(scale.shape)}")
-    _check_cache(what, cache, cache, scale, scale, cache.shape[1], cache.shape[3], cache.shape[3], cache.shape[2])
+    _, heads, tokens, dim = cache.shape
+    _check_cache(what, cache, cache, scale, scale, heads, dim, dim, tokens)
     _check_int32(what, "pages", pages, 1)
     if dtype not in TYPES:
         _refuse(f"{what}: numbers of {dtype}")
     n = pages.shape[0]
-    out = torch.empty((n, *cache.shape[1:]), dtype=dtype, device=cache.device)
-    _on_current_device(cache, scale, pages)
-    ops.ptr(cache)
-    _bind()
+    total, heads, tokens, dim = cache.shape
+    out = torch.empty((n, heads, tokens, dim), dtype=dtype, device=cache.device)
+    stream = launch_stream(cache.get_device(), scale, pages)
+    if _read is None:
+        _bind()
     for a in range(0, n, 65535):
         b = min(n, a + 65535)
-        ops.check(_read(ops.ptr(out[a:b]), ops.dtype_code(out), ops.ptr(cache), ops.ptr(scale), ops.ptr(pages[a:b]), b - a, cache.shape[0], cache.shape[1],
-                        cache.shape[3], ops.stream()))
+        to, ids = (out, pages) if b - a == n else (out[a:b], pages[a:b])
+        ops.check(_read(to.data_ptr(), ops.dtype_code(out), cache.data_ptr(), scale.data_ptr(), ids.data_ptr(), b - a, total, heads, dim, stream))
     return out
 
 
 def _check_attention(what, q, n_heads, n_kv_heads, head_dim, window, page_table, page_tokens, k_cache, v_cache, k_scale, v_scale, status, out, dv, softcap,
                      chunk, keep_first, sink, out_dtype):
-    """(rows, the output tensor) of a checked call."""
-    _check_cache(what, k_cache, v_cache, k_scale, v_scale, n_kv_heads, head_dim, dv, page_tokens)
+    """(rows, pages, the output tensor) of a checked call."""
+    n_pages = _check_cache(what, k_cache, v_cache, k_scale, v_scale, n_kv_heads, head_dim, dv, page_tokens)
     T, wq, _ = ops._rows(q)
-    if q.dtype not in TYPES or n_heads < 1 or n_heads % n_kv_heads or wq != n_heads * head_dim:
+    dtype = q.dtype
+    if dtype not in TYPES or n_heads < 1 or n_heads % n_kv_heads or wq != n_heads * head_dim:
         _refuse(f"{what}: queries {q.dtype} {tuple(q.shape)} of {n_heads} heads of {head_dim} over {n_kv_heads} key heads")
     if head_dim > 512 or dv > 512:
         _refuse(f"{what}: head sizes {head_dim} and {dv} (up to 512)")
@@ -143,8 +157,8 @@ def _check_attention(what, q, n_heads, n_kv_heads, head_dim, window, page_table,
         _refuse(f"{what}: scores capped at {softcap}")
     if sink is not None and (sink.dtype != torch.float32 or sink.numel() != n_heads or not sink.is_contiguous()):
         _refuse(f"{what}: sinks are contiguous float32 [{n_heads}], got {sink.dtype} {tuple(sink.shape)}")
-    want = out.dtype if out is not None else out_dtype or q.dtype
-    if want not in ((torch.float32,) if q.dtype == torch.float32 else TYPES) or (out is not None and out_dtype not in (None, out.dtype)):
+    want = out.dtype if out is not None else out_dtype or dtype
+    if want not in TYPES or (dtype is torch.float32 and want is not dtype) or (out is not None and out_dtype not in (None, want)):
         _refuse(f"{what}: a result of {want} from queries of {q.dtype}")
     if out is None:
         out = torch.empty((T, n_heads * dv), dtype=want, device=q.device)
@@ -152,7 +166,7 @@ def _check_attention(what, q, n_heads, n_kv_heads, head_dim, window, page_table,
         _refuse(f"{what}: the output view {tuple(out.shape)} does not fit")
     _check_int32(what, "page_table", page_table, 2)
     _check_status(what, status)
-    return T, out
+    return T, n_pages, out
 
 
 def decode(q, n_heads, n_kv_heads, head_dim, scale, window, tok_slot, tok_pos, page_table, page_tokens, k_cache, v_cache, k_scale, v_scale,
@@ -163,7 +177,7 @@ def decode(q, n_heads, n_kv_heads, head_dim, scale, window, tok_slot, tok_pos, p
     gives zeros and status 1, a page its sequence does not hold status 3.  Rows with a slot below 0 give zeros."""
     what = "kv8.decode"
     dv = int(v_head_dim or head_dim)
-    T, out = _check_attention(what, q, n_heads, n_kv_heads, head_dim, window, page_table, page_tokens, k_cache, v_cache, k_scale, v_scale, status, out, dv,
+    T, n_pages, out = _check_attention(what, q, n_heads, n_kv_heads, head_dim, window, page_table, page_tokens, k_cache, v_cache, k_scale, v_scale, status, out, dv,
                               softcap, chunk, keep_first, sink, out_dtype)
     _check_int32(what, "tok_slot", tok_slot, 1, T)
     _check_int32(what, "tok_pos", tok_pos, 1, T)
@@ -171,25 +185,27 @@ def decode(q, n_heads, n_kv_heads, head_dim, scale, window, tok_slot, tok_pos, p
         _refuse(f"{what}: a context of {max_context}")
     if T == 0:
         return out
-    _on_current_device(q, out, tok_slot, tok_pos, page_table, k_cache, v_cache, k_scale, v_scale, status, sink)
-    ops.ptr(q)
-    _bind()
+    stream = launch_stream(q.get_device(), out, tok_slot, tok_pos, page_table, k_cache, v_cache, k_scale, v_scale, status, sink)
+    if _decode is None:
+        _bind()
+    slots, max_pages = page_table.shape
+    code, wide = ops.dtype_code(q), out.dtype is torch.float32
+    cache = k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr()
     if head_dim % 16 == 0 and dv % 16 == 0 and head_dim <= 256 and dv <= 256 and T <= 65535 and max_context <= MAX_SPLIT_CONTEXT:
         floats = _scratch(T, n_heads, head_dim, dv, max_context)
-        partial = torch.empty((floats,), dtype=torch.float32, device=q.device) if floats else None
-        ops.check(_decode(ops.ptr(out), int(out.dtype == torch.float32), out.stride(0), ops.ptr(q), ops.dtype_code(q), q.stride(0), T, ops.ptr(tok_slot), ops.ptr(tok_pos),
-                          ops.ptr(page_table), page_table.shape[0], page_table.shape[1], k_cache.shape[0], ops.ptr(k_cache), ops.ptr(v_cache), ops.ptr(k_scale),
-                          ops.ptr(v_scale), n_heads, n_kv_heads, head_dim, dv, float(scale), int(window), int(chunk), int(keep_first), ops.ptr(sink),
-                          float(softcap or 0.0), int(max_context), ops.ptr(partial), ops.ptr(status), ops.stream()))
-        if partial is not None:
+        partial = None
+        if floats:
+            partial = torch.empty((floats,), dtype=torch.float32, device=q.device)
             ops.count_launches(1)                       # split kernel + merge kernel
+        ops.check(_decode(out.data_ptr(), 1 if wide else 0, out.stride(0), q.data_ptr(), code, q.stride(0), T, tok_slot.data_ptr(), tok_pos.data_ptr(),
+                          page_table.data_ptr(), slots, max_pages, n_pages, *cache, n_heads, n_kv_heads, head_dim, dv, float(scale), int(window), int(chunk),
+                          int(keep_first), _at(sink), float(softcap or 0.0), int(max_context), _at(partial), status.data_ptr(), stream))
         return out
     for a in range(0, T, 65535):
         b = min(T, a + 65535)
-        ops.check(_attention(ops.ptr(out[a:b]), ops.dtype_code(out), out.stride(0), ops.ptr(q[a:b]), ops.dtype_code(q), q.stride(0), b - a, ops.ptr(tok_slot[a:b]),
-                             ops.ptr(tok_pos[a:b]), None, 0, ops.ptr(page_table), page_table.shape[0], page_table.shape[1], k_cache.shape[0], ops.ptr(k_cache),
-                             ops.ptr(v_cache), ops.ptr(k_scale), ops.ptr(v_scale), n_heads, n_kv_heads, head_dim, dv, float(scale), int(window), int(chunk),
-                             int(keep_first), ops.ptr(sink), float(softcap or 0.0), int(max_context), ops.ptr(status), ops.stream()))
+        ops.check(_attention(out[a:b].data_ptr(), ops.F32 if wide else ops.BF16, out.stride(0), q[a:b].data_ptr(), code, q.stride(0), b - a, tok_slot[a:b].data_ptr(),
+                             tok_pos[a:b].data_ptr(), None, 0, page_table.data_ptr(), slots, max_pages, n_pages, *cache, n_heads, n_kv_heads, head_dim, dv,
+                             float(scale), int(window), int(chunk), int(keep_first), _at(sink), float(softcap or 0.0), int(max_context), status.data_ptr(), stream))
     return out
 
 
@@ -199,30 +215,30 @@ def prefill(q, n_heads, n_kv_heads, head_dim, scale, window, tiles, page_table, 
     slot) as from `attention_bf16.prefill_tiles`; rows that no tile covers are left as they are, or zeros with `padded`.  The rest as for `decode`."""
     what = "kv8.prefill"
     dv = int(v_head_dim or head_dim)
-    T, out = _check_attention(what, q, n_heads, n_kv_heads, head_dim, window, page_table, page_tokens, k_cache, v_cache, k_scale, v_scale, status, out, dv,
+    T, n_pages, out = _check_attention(what, q, n_heads, n_kv_heads, head_dim, window, page_table, page_tokens, k_cache, v_cache, k_scale, v_scale, status, out, dv,
                               softcap, chunk, keep_first, sink, out_dtype)
     _check_int32(what, "tiles", tiles, 2)
     if tiles.shape[1] != 4:
         _refuse(f"{what}: tiles are [n, 4], got {tuple(tiles.shape)}")
     if T == 0:
         return out
-    _on_current_device(q, out, tiles, page_table, k_cache, v_cache, k_scale, v_scale, status, sink)
-    ops.ptr(q)
-    _bind()
+    stream = launch_stream(q.get_device(), out, tiles, page_table, k_cache, v_cache, k_scale, v_scale, status, sink)
+    if _prefill is None:
+        _bind()
     if padded:
         out.zero_()
-    wide = int(out.dtype == torch.float32)
-    if (q.dtype == torch.bfloat16 and head_dim % 16 == 0 and dv % 16 == 0 and head_dim <= 256 and dv <= 256 and scale > 0 and tiles.shape[0] <= 65535
+    slots, max_pages = page_table.shape
+    n, code, wide = tiles.shape[0], ops.dtype_code(q), out.dtype is torch.float32
+    cache = k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr()
+    if (code == ops.BF16 and head_dim % 16 == 0 and dv % 16 == 0 and head_dim <= 256 and dv <= 256 and scale > 0 and n <= 65535
             and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0 and out.stride(0) % (4 if wide else 8) == 0 and out.data_ptr() % 16 == 0):
-        ops.check(_prefill(ops.ptr(out), wide, out.stride(0), ops.ptr(q), q.stride(0), T, ops.ptr(k_cache), ops.ptr(v_cache), ops.ptr(k_scale), ops.ptr(v_scale),
-                           k_cache.shape[0], ops.ptr(page_table), page_table.shape[0], page_table.shape[1], ops.ptr(tiles), tiles.shape[0], n_heads, n_kv_heads,
-                           head_dim, dv, float(scale), int(window), int(chunk), int(keep_first), ops.ptr(sink), float(softcap or 0.0), ops.ptr(status),
-                           ops.stream()))
+        ops.check(_prefill(out.data_ptr(), 1 if wide else 0, out.stride(0), q.data_ptr(), q.stride(0), T, *cache, n_pages, page_table.data_ptr(), slots, max_pages,
+                           tiles.data_ptr(), n, n_heads, n_kv_heads, head_dim, dv, float(scale), int(window), int(chunk), int(keep_first), _at(sink),
+                           float(softcap or 0.0), status.data_ptr(), stream))
         return out
-    for a in range(0, tiles.shape[0], 511):
-        b = min(tiles.shape[0], a + 511)
-        ops.check(_attention(ops.ptr(out), ops.dtype_code(out), out.stride(0), ops.ptr(q), ops.dtype_code(q), q.stride(0), T, None, None, ops.ptr(tiles[a:b]), b - a,
-                             ops.ptr(page_table), page_table.shape[0], page_table.shape[1], k_cache.shape[0], ops.ptr(k_cache), ops.ptr(v_cache),
-                             ops.ptr(k_scale), ops.ptr(v_scale), n_heads, n_kv_heads, head_dim, dv, float(scale), int(window), int(chunk), int(keep_first),
-                             ops.ptr(sink), float(softcap or 0.0), 2147483647, ops.ptr(status), ops.stream()))
+    for a in range(0, n, 511):
+        b = min(n, a + 511)
+        ops.check(_attention(out.data_ptr(), ops.F32 if wide else ops.BF16, out.stride(0), q.data_ptr(), code, q.stride(0), T, None, None, tiles[a:b].data_ptr(), b - a,
+                             page_table.data_ptr(), slots, max_pages, n_pages, *cache, n_heads, n_kv_heads, head_dim, dv, float(scale), int(window), int(chunk),
+                             int(keep_first), _at(sink), float(softcap or 0.0), 2147483647, status.data_ptr(), stream))
     return out

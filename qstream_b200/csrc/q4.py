@@ -9,7 +9,6 @@ from __future__ import annotations
 
 import functools
 from ctypes import c_int, c_longlong, c_void_p
-from dataclasses import dataclass
 
 import torch
 
@@ -37,7 +36,6 @@ def _refuse(text, code=QsError.INVALID_INPUT):
     raise QStreamError(code, text)
 
 
-@dataclass(frozen=True)
 class Weight4:
     """A matrix [out_features, in_features] in 4 bits.
 
@@ -45,22 +43,21 @@ class Weight4:
     2 h + u holds row g + 8 u of the tile, columns 32 h + 8 t + (0, 2, 4, 6, 1, 3, 5, 7), lowest four bits first.
     scales: bfloat16 [ceil(out / 16)][groups][8][2], entry (g, u) for row g + 8 u; groups cover the columns rounded up to 64.
     What fills up the last rows and columns are codes of 8 and scales of 0."""
-    codes: torch.Tensor
-    scales: torch.Tensor
-    out_features: int
-    in_features: int
-    group: int
+    __slots__ = ("codes", "scales", "out_features", "in_features", "group", "_at")
 
-    def __post_init__(self):
-        n, k, g = self.out_features, self.in_features, self.group
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, out_features: int, in_features: int, group: int):
+        n, k, g = self.out_features, self.in_features, self.group = out_features, in_features, group
+        self.codes, self.scales = codes, scales
         if n < 1 or k < 1 or g not in GROUPS:
             _refuse(f"4-bit weights: a matrix [{n}, {k}] in groups of {g} (groups: {GROUPS})", QsError.QUANT_MISMATCH)
         tiles, chunks = -(-n // 16), -(-k // 64)
-        want = (tiles, chunks, 32, 16), (tiles, -(-chunks * 64 // g), 8, 2)
-        for name, t, shape, dtype in (("codes", self.codes, want[0], torch.uint8), ("scales", self.scales, want[1], torch.bfloat16)):
-            if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous():
-                _refuse(f"4-bit weights: {name} of [{n}, {k}] in groups of {g} are contiguous {dtype} {shape}, got {t.dtype} {tuple(t.shape)}", QsError.QUANT_MISMATCH)
-        if self.codes.device != self.scales.device or self.codes.data_ptr() % 16 or self.scales.data_ptr() % 4:
+        if codes.shape != (tiles, chunks, 32, 16) or codes.dtype is not torch.uint8 or not codes.is_contiguous() \
+                or scales.shape != (tiles, -(-chunks * 64 // g), 8, 2) or scales.dtype is not torch.bfloat16 or not scales.is_contiguous():
+            _refuse(f"4-bit weights: [{n}, {k}] in groups of {g} are contiguous uint8 codes and bfloat16 scales of {sizes(n, k, g)}, got {codes.dtype} "
+                    f"{tuple(codes.shape)} and {scales.dtype} {tuple(scales.shape)}", QsError.QUANT_MISMATCH)
+        # (device, addresses) for the calls
+        self._at = codes.get_device(), codes.data_ptr(), scales.data_ptr()
+        if scales.get_device() != self._at[0] or self._at[1] % 16 or self._at[2] % 4:
             _refuse("4-bit weights: codes and scales lie on one device, the codes on a 16-byte boundary")
 
     @property
@@ -85,14 +82,16 @@ def sizes(out_features: int, in_features: int, group: int):
     return (tiles, chunks, 32, 16), (tiles, -(-chunks * 64 // group), 8, 2)
 
 
-def _on_current_device(*tensors):
-    """All operands on the device whose stream the kernels are launched on."""
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) > 1:
-        _refuse(f"operands on several devices: {sorted(map(str, devices))}")
-    device = devices.pop()
-    if device.type == "cuda" and device.index != torch.cuda.current_device():
-        _refuse(f"operands on {device}, but the current device is cuda:{torch.cuda.current_device()}")
+def launch_stream(device: int, *tensors) -> int:
+    """The stream to launch on, for operands that all lie on the current device (`device`: the first one's index, -1 on the host)."""
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            _refuse(f"operands on several devices: one on {t.device}, others on {'cuda:%d' % device if device >= 0 else 'the host'}")
+    if device < 0:
+        _refuse("kernels run on CUDA tensors only; there is no CPU path")
+    if device != torch.cuda.current_device():
+        _refuse(f"operands on cuda:{device}, but the current device is cuda:{torch.cuda.current_device()}")
+    return ops.stream()
 
 
 def quantize(weight: torch.Tensor, group: int = 64) -> Weight4:
@@ -102,14 +101,13 @@ def quantize(weight: torch.Tensor, group: int = 64) -> Weight4:
         _refuse(f"4-bit weights: need a float32 or bfloat16 matrix with contiguous rows, got {weight.dtype} {tuple(weight.shape)} strides {weight.stride()}")
     if group not in GROUPS:
         _refuse(f"4-bit weights: groups of {group} columns (groups: {GROUPS})", QsError.QUANT_MISMATCH)
-    ops.ptr(weight)
-    _on_current_device(weight)
+    stream = launch_stream(weight.get_device())
     _bind()
     N, K = weight.shape
     shapes = sizes(N, K, group)
     codes = torch.empty(shapes[0], dtype=torch.uint8, device=weight.device)
     scales = torch.zeros(shapes[1], dtype=torch.bfloat16, device=weight.device)
-    ops.check(_quantize(ops.ptr(codes), ops.ptr(scales), ops.ptr(weight), ops.dtype_code(weight), weight.stride(0), N, K, group, ops.stream()))
+    ops.check(_quantize(ops.ptr(codes), ops.ptr(scales), ops.ptr(weight), ops.dtype_code(weight), weight.stride(0), N, K, group, stream))
     return Weight4(codes, scales, N, K, group)
 
 
@@ -119,33 +117,43 @@ def linear(x, weight: Weight4, bias=None, activation=None, residuals=(), out_dty
     write into (contiguous rows, any row stride).  `settled`: the weight was complete before the previous kernel of the stream began
     (a model's is); the kernel then fetches it while that kernel still runs."""
     M, K, ldx = ops._rows(x)
-    N = weight.out_features
+    N, dtype = weight.out_features, x.dtype
+    wide = dtype is torch.float32
     if K != weight.in_features:
         _refuse(f"linear: x is [{M}, {K}] but weight is {weight.shape}")
-    if x.dtype not in TYPES:
-        _refuse(f"linear: rows of {x.dtype}; 4-bit weights take float32 or bfloat16")
-    if activation not in ops.ACTIVATIONS:
-        _refuse(f"linear: activation '{activation}' has no kernel")
-    if bias is not None and (bias.dim() != 1 or bias.numel() != N or bias.stride(0) != 1 or bias.dtype not in TYPES):
-        _refuse(f"linear: a bias for {N} results, got {bias.dtype} {tuple(bias.shape)}")
-    want = out.dtype if out is not None else out_dtype or x.dtype
-    if want not in ((torch.float32,) if x.dtype == torch.float32 else TYPES) or (out is not None and out_dtype not in (None, out.dtype)):
-        _refuse(f"linear: a result of {want} from rows of {x.dtype}")
+    if not wide and dtype is not torch.bfloat16:
+        _refuse(f"linear: rows of {dtype}; 4-bit weights take float32 or bfloat16")
     if K > MAX_COLUMNS:
         _refuse(f"linear: {K} columns, the kernels take {MAX_COLUMNS}")
-    out, res, ldr = ops._product_views(x, M, N, [r for r in residuals if r is not None], want, out)
+    act = ops.ACTIVATIONS.get(activation)
+    if act is None:
+        _refuse(f"linear: activation '{activation}' has no kernel")
+    if bias is not None and (bias.shape != (N,) or bias.stride(0) != 1 or bias.dtype not in TYPES):
+        _refuse(f"linear: a bias for {N} results, got {bias.dtype} {tuple(bias.shape)}")
+    want = out.dtype if out is not None else out_dtype or dtype
+    if want not in TYPES or (wide and want is not torch.float32) or (out is not None and out_dtype not in (None, want)):
+        _refuse(f"linear: a result of {want} from rows of {dtype}")
+    if residuals or out is not None:
+        out, res, ldr = ops._product_views(x, M, N, [r for r in residuals if r is not None], want, out)
+        r0, r1 = res[:2]
+    else:
+        out, r0, r1, ldr = torch.empty((M, N), dtype=want, device=x.device), None, None, N
     if M == 0:
         return out
-    _on_current_device(x, weight.codes, bias, out, *res[:2])
-    _bind()
-    code, element = ops.dtype_code(x), x.element_size()
-    aligned = x.data_ptr() % 16 == 0 and ldx * element % 16 == 0
-    nbytes = _scratch(M, N, K, code, int(aligned))          # rows laid out anew, for many rows the operands' powers of two
-    scratch = torch.empty((nbytes,), dtype=torch.uint8, device=x.device) if nbytes else None
-    if nbytes:
-        ops.count_launches(_kernels(M, N, K, code, int(aligned)) - 1)
-    ops.check(_linear(ops.ptr(out), ops.dtype_code(out), out.stride(0), ops.ptr(x), code, ldx, int(aligned), ops.ptr(weight.codes), ops.ptr(weight.scales),
-                      ops.ptr(bias), ops.dtype_code(bias) if bias is not None else 0, ops.ACTIVATIONS[activation], ops.ptr(res[0]), ops.ptr(res[1]), ldr,
-                      M, N, K, weight.group, int(bool(settled)), ops.ptr(scratch),
-                      ops.ptr(gemm_tc.status_word(x.device)), ops.stream()))
+    device, codes, scales = weight._at
+    stream = launch_stream(device, x, bias, out, r0, r1)
+    if _linear is None:
+        _bind()
+    code, at = (ops.F32, x.data_ptr()) if wide else (ops.BF16, x.data_ptr())
+    aligned = int(at % 16 == 0 and ldx % (4 if wide else 8) == 0)
+    scratch = None
+    if wide or M > 16 or K % 64 or not aligned:             # rows laid out anew; for many rows the operands' powers of two
+        nbytes = _scratch(M, N, K, code, aligned)
+        if nbytes:
+            scratch = torch.empty((nbytes,), dtype=torch.uint8, device=x.device)
+            ops.count_launches(_kernels(M, N, K, code, aligned) - 1)
+    ops.check(_linear(out.data_ptr(), ops.F32 if want is torch.float32 else ops.BF16, out.stride(0), at, code, ldx, aligned, codes, scales,
+                      None if bias is None else bias.data_ptr(), 0 if bias is None else ops.dtype_code(bias), act, None if r0 is None else r0.data_ptr(),
+                      None if r1 is None else r1.data_ptr(), ldr, M, N, K, weight.group, 1 if settled else 0, None if scratch is None else scratch.data_ptr(),
+                      gemm_tc.status_word(x.device).data_ptr(), stream))
     return out

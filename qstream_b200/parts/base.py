@@ -66,7 +66,7 @@ class Runtime:
     dtype: torch.dtype                  # storage type of activations: bfloat16 or float32
     device: torch.device
     weight_group: int = 0               # g > 0: the matrices of attention and dense feed-forwards in 4 bits, a scale for each g columns
-    narrowed: list = field(default_factory=list)        # (bytes before, bytes after) of every matrix that `matrix` rounded
+    narrowed: list = field(default_factory=list, compare=False)        # (bytes before, bytes after) of every matrix that `matrix` rounded
 
     def matrix(self, weight: torch.Tensor):
         """A part's matrix as its products take it: as it is, or rounded to 4 bits."""

@@ -54,7 +54,7 @@ CACHE = dict(k_cache=torch.zeros(5, 2, 64, 16, dtype=torch.int8), v_cache=torch.
 BAD_CACHE = [dict(k_cache=CACHE["k_cache"].short()), dict(k_cache=CACHE["k_cache"][:, :1]), dict(k_cache=CACHE["k_cache"][:4]), dict(v_cache=CACHE["v_cache"][..., :7]),
              dict(k_scale=torch.zeros(5, 3)), dict(v_scale=torch.zeros(5, 2).double()), dict(k_scale=torch.zeros(2, 5).t()), dict(page_tokens=32),
              dict(k_cache=CACHE["k_cache"][:0], v_cache=CACHE["v_cache"][:0], k_scale=torch.zeros(0, 2), v_scale=torch.zeros(0, 2)), dict(page_table=I(2, 3).long()),
-             dict(page_table=I(6)), dict(page_table=I(0, 3)), dict(status=torch.zeros(1)), dict(status=I(0))]
+             dict(n_kv_heads=0, **{n: t[:, :0] for n, t in CACHE.items()}), dict(page_table=I(6)), dict(page_table=I(0, 3)), dict(status=torch.zeros(1)), dict(status=I(0))]
 
 
 def test_writes_that_are_refused():
