@@ -17,7 +17,8 @@
 //   warp 0          copies the rows of x (TMA)
 //   warp 1          multiplies (tcgen05.mma, D [128 x rows of x], 32-bit, in TMEM)
 // In the end D goes through shared memory, so that a warp finishes whole rows of results.
-// Bound by shared memory: a chunk is 16 KB written and read for each operand, 512 cycles where the product takes 256.
+// Bound by the hand-over of stages: of a stage's 1,000 cycles the thread that multiplies waits for its barrier or issues, where the products
+// themselves take 512 (and shared memory's traffic, 32 KB written and read for each chunk, about as much).
 //
 // Where blocks are few, those of a cluster share the columns, and add their sums through distributed shared memory, in their order.
 #include "common.cuh"
@@ -224,10 +225,12 @@ q4_many_kernel(const __grid_constant__ CUtensorMap map_x, const Many p) {
             const int i = i0 + turn * TEAMS;
             if (i >= 2 * pairs) break;
             const int pair = i >> 1, st = pair % STAGES, slot = i / SLOT_CHUNKS % SLOTS;
-            if (i >= n) { mbar_arrive(&full[st]); break; }     // half a stage at the end: nothing to write
-            if (!mbar_wait(&c_full[slot], (i / SLOT_CHUNKS / SLOTS) & 1)) ok = false;
+            if (i < n && !mbar_wait(&c_full[slot], (i / SLOT_CHUNKS / SLOTS) & 1)) ok = false;
             if (ok && (aborted || !mbar_wait(&empty[st], ((pair / STAGES) & 1) ^ 1))) ok = false;
             if (!ok) { if (lane == 0) atomicExch(p.status, 133); aborted = 1; break; }
+            // Half a stage at the end has nothing to write, but its arrival is for this phase too: not before the stage is free, or the stage's last
+            // phase, still short of others, would count it.
+            if (i >= n) { mbar_arrive(&full[st]); break; }
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
                 uint32_t unit[PER][2];

@@ -173,6 +173,19 @@ def test_many_columns(n, k):
             assert (np.abs(U.f64(q4.linear(x, w)) - want) <= bound).all(), m
 
 
+@pytest.mark.parametrize("m,n,chunks", [(200, 2000, 47), (17, 9500, 93), (130, 20000, 5), (700, 1000, 23), (300, 19000, 7)])
+def test_products_of_many_rows_whose_blocks_end_on_half_a_stage(m, n, chunks):
+    """An odd number of chunks of 64 columns leaves half of a block's last stage unwritten; again and again, the same bits."""
+    k = 64 * chunks
+    w = q4.quantize(normal(n + k, n, k, std=0.05), 64)
+    x = normal(m, m, k, dtype=torch.bfloat16)
+    first = q4.linear(x, w)
+    want, bound = U.linear(U.f64(x), U.dense(w), out_bf16=True)
+    assert (np.abs(U.f64(first) - want) <= bound).all()
+    for _ in range(100):
+        assert torch.equal(q4.linear(x, w), first)
+
+
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("m,n,k", [(17, 6000, 6016), (130, 2100, 2500), (300, 1000, 2048), (33, 1100, 17000), (1000, 130, 4800), (3000, 16, 12800)])
 def test_products_of_many_rows(m, n, k, group):
