@@ -2,9 +2,11 @@
 //
 //   s[u] = scale * q.K[u] (capped), K[u] = code * scale of u's page;  softmax over the keys that the mask leaves;  o = sum_u p[u] V[u]
 //
-// Bound by the bytes of the pages.  A warp takes 32 keys (16 of wide heads) and up to HEADS query heads that share their key head: a bulk
+// Floor: the bytes of the pages.  A warp takes 32 keys and up to HEADS query heads that share their key head: a bulk
 // copy brings the keys into shared memory, asynchronous copies the values, their rows apart (all of a block are on their way at once, from
-// the first instructions on); 16-bit products on mma.m16n8k16 take them from there.
+// the first instructions on); 16-bit products on mma.m16n8k16 take them from there.  Bound by a block's life: its metadata's and pages' way from
+// memory, one behind the other, then instructions, which fill two fifths of the slots.  (Blocks that stay on their SM and look for their next
+// page's number beside the products: 31 rows of 2,048 29 us instead of 25 without the merge; they wait and compute all at the same time.)
 //
 //   scores   left operand: 16 keys, right: the heads.  A lane's 16 bytes of a key's row are its part of four steps; which dims meet in
 //            a step is free, so the queries are laid out the same way.  A code, as the low byte of a 16-bit float 1024 beside its upper
@@ -28,7 +30,7 @@
 
 namespace {
 
-constexpr int PAGE = 64, WARPS = 8;
+constexpr int PAGE = 64, KEYS = 32;                     // of a page; of a warp
 
 struct DecodeArgs {
     void* out;
@@ -102,9 +104,9 @@ __device__ __forceinline__ void store_places(void* out, int type, size_t at, flo
     }
 }
 
-// KC: blocks of 64 dims that keys span at most; VB: blocks of 128 dims of the values; a warp takes KEYS keys.  FULL: keys and values fill the
+// KC: blocks of 64 dims that keys span at most; VB: blocks of 128 dims of the values; a block has WARPS warps.  FULL: keys and values fill the
 // blocks (addresses are then constants apart).
-template <typename T, int KC, int VB, int KEYS, bool FULL>
+template <typename T, int KC, int VB, int WARPS, bool FULL>
 __global__ void __launch_bounds__(WARPS * 32)
 kv8_decode_kernel(const DecodeArgs p) {
     constexpr bool WIDE = sizeof(T) == 4;                // two columns to a head
@@ -129,13 +131,15 @@ kv8_decode_kernel(const DecodeArgs p) {
     const int slot = p.tok_slot[row], pos = p.tok_pos[row];
     // The queries, laid out for all warps: warp w makes column w, which is head w (WIDE: head w & 3, its first or second term); lane l
     // its dims 8 l .. 8 l + 7.  A lane of the products has dims 64 c + 16 t .. + 15 of column g.  Their way from memory runs beside that of the step's metadata.
-    float x[8];
-    {
-        const T* src = reinterpret_cast<const T*>(p.q) + (size_t)row * p.ldq + (size_t)(head0 + min(WIDE ? warp & 3 : warp, heads - 1)) * dk + 8 * lane;
-        if (8 * lane < dk && p.q_aligned) load8_as_f32(src, WIDE ? QS_F32 : QS_BF16, 0, x);
+    float x[8 / WARPS][8];
+#pragma unroll
+    for (int c = 0; c < 8 / WARPS; ++c) {
+        const int column = warp + c * WARPS;
+        const T* src = reinterpret_cast<const T*>(p.q) + (size_t)row * p.ldq + (size_t)(head0 + min(WIDE ? column & 3 : column, heads - 1)) * dk + 8 * lane;
+        if (8 * lane < dk && p.q_aligned) load8_as_f32(src, WIDE ? QS_F32 : QS_BF16, 0, x[c]);
         else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = 8 * lane + i < dk ? to_f32(src[i]) : 0.f;
+            for (int i = 0; i < 8; ++i) x[c][i] = 8 * lane + i < dk ? to_f32(src[i]) : 0.f;
         }
     }
     if (slot < 0 || slot >= p.n_slots || pos < 0 || (pos >> 6) >= p.max_pages || pos >= p.splits * SPLIT) {
@@ -179,23 +183,25 @@ kv8_decode_kernel(const DecodeArgs p) {
         asm volatile("ld.global.f32 %0, [%1];" : "=f"(vs) : "l"(p.v_scale + at));
     }
 
-    {
+#pragma unroll
+    for (int c = 0; c < 8 / WARPS; ++c) {
+        const int column = warp + c * WARPS;
         float most = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[i]));
+        for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[c][i]));
         most = warp_max(most);
         // the power of two at or below the largest; numbers that are not finite go through as they are
         const uint32_t e = min(max(__float_as_uint(most) >> 23, 1u), 253u);
         const float inv = __uint_as_float((254u - e) << 23);
-        if (lane == 0) s_unit[warp] = __uint_as_float(e << 23);
+        if (lane == 0) s_unit[column] = __uint_as_float(e << 23);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            uint32_t v = pack_f16(x[2 * i] * inv, x[2 * i + 1] * inv);
-            if (WIDE && warp >= 4) {
+            uint32_t v = pack_f16(x[c][2 * i] * inv, x[c][2 * i + 1] * inv);
+            if (WIDE && column >= 4) {
                 const float2 hi = unpack_f16(v);
-                v = pack_f16(x[2 * i] * inv - hi.x, x[2 * i + 1] * inv - hi.y);
+                v = pack_f16(x[c][2 * i] * inv - hi.x, x[c][2 * i + 1] * inv - hi.y);
             }
-            if (lane < KC * 8) s_q[(lane >> 3) * 8 + (lane & 1) * 4 + i][warp * 4 + (lane >> 1 & 3)] = v;
+            if (lane < KC * 8) s_q[(lane >> 3) * 8 + (lane & 1) * 4 + i][column * 4 + (lane >> 1 & 3)] = v;
         }
     }
     __syncthreads();
@@ -390,7 +396,11 @@ kv8_merge_kernel(const DecodeArgs p) {
     grid_dep_wait();
     const int head = blockIdx.x, row = blockIdx.y, dv = p.dv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int slot = p.tok_slot[row], pos = p.tok_pos[row], type = p.out_f32 ? QS_F32 : QS_BF16;
-    const size_t to = (size_t)row * p.ldo + (size_t)head * dv;
+    const size_t to = (size_t)row * p.ldo + (size_t)head * dv, cell = ((size_t)row * p.n_heads + head) * p.splits;
+    // On the way beside the row's metadata, whether its splits turn out to be seen or not.
+    float2 ml = make_float2(0.f, 0.f);
+    if ((int)threadIdx.x < p.splits) asm volatile("ld.global.v2.f32 {%0, %1}, [%2];" : "=f"(ml.x), "=f"(ml.y) : "l"(p.ml + cell + threadIdx.x));
+    const float sink = p.sink ? p.sink[head] * 1.4426950408889634f : -INFINITY;
     if (slot < 0 || slot >= p.n_slots || pos < 0 || (pos >> 6) >= p.max_pages || pos >= p.splits * SPLIT) {       // padding, or reported: a defined row
         for (int d = threadIdx.x; d < dv; d += MERGE_THREADS) store_from_f32(p.out, type, to + d, 0.f);
         return;
@@ -398,26 +408,27 @@ kv8_merge_kernel(const DecodeArgs p) {
     const int first = first_key(p, pos), keep = p.window > 0 ? min(p.keep_first, first) : 0;
     // the splits with keys that are seen: those of the kept first keys, then those of the window
     const int kept = keep > 0 ? (keep - 1) / SPLIT + 1 : 0, lo = max(first / SPLIT, kept), n = kept + pos / SPLIT - lo + 1;
-    const size_t cell = ((size_t)row * p.n_heads + head) * p.splits;
     auto split = [&](int i) { return i < kept ? i : lo + i - kept; };
-    float M = p.sink ? p.sink[head] * 1.4426950408889634f : -INFINITY, L = 0.f;
-    for (int i = threadIdx.x; i < n; i += MERGE_THREADS) {
-        const float m = p.ml[cell + split(i)].x;
-        s_w[i] = m;
-        M = fmaxf(M, m);
-    }
+    auto seen = [&](int u) { return u < kept || (u >= lo && u < lo + n - kept); };
+    const bool mine = seen(threadIdx.x);
+    float M = mine ? fmaxf(sink, ml.x) : sink, L = 0.f;
+    for (int u = threadIdx.x + MERGE_THREADS; u < lo + n - kept; u += MERGE_THREADS)
+        if (seen(u)) M = fmaxf(M, p.ml[cell + u].x);
     M = warp_max(M);
     if (lane == 0) scratch[warp] = M;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < MERGE_THREADS / 32; ++i) M = fmaxf(M, scratch[i]);
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += MERGE_THREADS) {
-        s_w[i] = s_w[i] == -INFINITY ? 1.f : exp2f(s_w[i] - M);
-        L = fmaf(p.ml[cell + split(i)].y, s_w[i], L);
-    }
+    auto weigh = [&](int u, float2 ml) {
+        s_w[u] = ml.x == -INFINITY ? 1.f : exp2f(ml.x - M);
+        L = fmaf(ml.y, s_w[u], L);
+    };
+    if (mine) weigh(threadIdx.x, ml);
+    for (int u = threadIdx.x + MERGE_THREADS; u < lo + n - kept; u += MERGE_THREADS)
+        if (seen(u)) weigh(u, p.ml[cell + u]);
     L = block_sum(L, scratch);                           // (a barrier: the weights are there)
-    if (p.sink) L += exp2f(p.sink[head] * 1.4426950408889634f - M + 15.f);
+    if (p.sink) L += exp2f(sink - M + 15.f);
     const float inv = L != 0.f ? 1.0f / L : 0.f;
     constexpr int width = PLACES / 4, groups = MERGE_THREADS / width;
     const int group = threadIdx.x / width, place = threadIdx.x % width * 4, d = dim_of(place);
@@ -432,7 +443,7 @@ kv8_merge_kernel(const DecodeArgs p) {
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u)
             if (i0 + u < end) {
-                const float w = s_w[i0 + u];
+                const float w = s_w[split(i0 + u)];
                 o.x = fmaf(v[u].x, w, o.x); o.y = fmaf(v[u].y, w, o.y); o.z = fmaf(v[u].z, w, o.z); o.w = fmaf(v[u].w, w, o.w);
             }
     }
@@ -447,22 +458,24 @@ kv8_merge_kernel(const DecodeArgs p) {
     }
 }
 
-// Keys of a block: 256, half as many where they are wide (a block's keys and values then fill as much shared memory as before).
-int split_keys(int dk, int dv) { return WARPS * (dk > 128 || dv > 128 ? 16 : 32); }
+// Keys of a block.  Wide ones have four warps: their keys and values fill as much shared memory as the others', three blocks to an SM.  (8 rows of 1,024,
+// heads of 256: 27 us; eight warps of 16 keys, so that 114 registers let two blocks onto an SM, and each query column has a warp: 31.  Heads of 128, 31 rows of 2,048
+// and one of 65,536: four warps of 64 keys 29.3 and 29.4 us, eight of 32 keys 29.6 and 28.0.)
+int split_keys(int dk, int dv) { return KEYS * (dk > 128 || dv > 128 ? 4 : 8); }
 
 // Places of a head's sums.
 int places(int dk, int dv) { return dk > 128 || dv > 128 ? 256 : 128; }
 
-template <typename T, int KC, int VB, int KEYS, bool FULL>
+template <typename T, int KC, int VB, int WARPS, bool FULL>
 int go(const DecodeArgs& p, int rows, cudaStream_t stream) {
     constexpr int HEADS = sizeof(T) == 4 ? 4 : 8;
     const int pages = WARPS * (KEYS * (p.dk + p.dv + 16) + 128), sums = WARPS * HEADS * (VB * 128 + 4) * 4, smem = pages > sums ? pages : sums;
     static PerDevice limit;
     int device = 0;
     cudaGetDevice(&device);
-    limit.get(device, [] { return cudaFuncSetAttribute(kv8_decode_kernel<T, KC, VB, KEYS, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024) == cudaSuccess ? 1 : 0; });
+    limit.get(device, [] { return cudaFuncSetAttribute(kv8_decode_kernel<T, KC, VB, WARPS, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024) == cudaSuccess ? 1 : 0; });
     const int per = p.n_heads / p.n_kv_heads;
-    cudaError_t e = qs_launch_dependent(kv8_decode_kernel<T, KC, VB, KEYS, FULL>, dim3(p.splits, p.n_kv_heads * ((per + HEADS - 1) / HEADS), rows), dim3(WARPS * 32), (size_t)smem, stream, p);
+    cudaError_t e = qs_launch_dependent(kv8_decode_kernel<T, KC, VB, WARPS, FULL>, dim3(p.splits, p.n_kv_heads * ((per + HEADS - 1) / HEADS), rows), dim3(WARPS * 32), (size_t)smem, stream, p);
     if (e == cudaSuccess && p.splits > 1)
         e = qs_launch_dependent(kv8_merge_kernel<WARPS * KEYS, VB * 128>, dim3(p.n_heads, rows), dim3(MERGE_THREADS), (size_t)p.splits * sizeof(float), stream, p);
     if (e != cudaSuccess) return qs_fail(QS_ERR_INTERNAL, "kv8 decode: %s", cudaGetErrorString(e));
@@ -502,11 +515,11 @@ QS_API int qs_kv8_decode(void* out, int out_f32, long long ldo, const void* q, i
     const DecodeArgs p = {out, partial, (float2*)(partial + (size_t)T_tokens * n_heads * splits * places(dk, dv)), q, k_cache, v_cache, k_scale, v_scale, sink, tok_slot, tok_pos, page_table, (size_t)ldo, (size_t)ldq,
                           max_pages, n_slots, n_pages, n_heads, n_kv_heads, dk, dv, window, chunk, keep_first, splits, out_f32, scale, softcap,
                           softcap > 0.f ? 2.f * 1.4426950408889634f / softcap : 0.f, q_aligned, status};
-#define GO(T) do { if (dk <= 64 && dv <= 128) return go<T, 1, 1, 32, false>(p, T_tokens, stream); \
-                   if (dk == 128 && dv == 128) return go<T, 2, 1, 32, true>(p, T_tokens, stream); \
-                   if (dk <= 128 && dv <= 128) return go<T, 2, 1, 32, false>(p, T_tokens, stream); \
-                   if (dk == 256 && dv == 256) return go<T, 4, 2, 16, true>(p, T_tokens, stream); \
-                   return go<T, 4, 2, 16, false>(p, T_tokens, stream); } while (0)
+#define GO(T) do { if (dk <= 64 && dv <= 128) return go<T, 1, 1, 8, false>(p, T_tokens, stream); \
+                   if (dk == 128 && dv == 128) return go<T, 2, 1, 8, true>(p, T_tokens, stream); \
+                   if (dk <= 128 && dv <= 128) return go<T, 2, 1, 8, false>(p, T_tokens, stream); \
+                   if (dk == 256 && dv == 256) return go<T, 4, 2, 4, true>(p, T_tokens, stream); \
+                   return go<T, 4, 2, 4, false>(p, T_tokens, stream); } while (0)
     if (dtype == QS_F32) GO(float);
     GO(__nv_bfloat16);
 #undef GO
