@@ -9,16 +9,18 @@
 // 64 columns: 700 rows, 8,192 x 2,048: 160 us, 33 rows, 4,096 x 16,384: 52.)
 //
 // A block takes 128 rows of the matrix and up to 128 rows of x.  Chunk by chunk of 64 columns:
-//   warp 18         copies the codes to shared memory, four chunks of eight tiles at a time (bulk copies)
-//   warps 2 .. 17   four teams, a chunk to each; a warp takes 32 rows: a code c, shifted into the lowest bits of a 16-bit 1024, is 1024 + c; 1032 less,
-//                   times the scale; a word of eight codes is one chunk of 16 bytes of a row in the layout of the 128-byte swizzle.  Lanes of
+//   warp 18         copies the codes to shared memory, four chunks of eight tiles at a time (TMA)
+//   warps 2 .. 17   four teams, a chunk to each; a warp takes 32 rows: a code c, shifted into the highest bits of a 16-bit 16, is 16 + c; a
+//                   multiply-add makes (c - 8) s of it; a word of eight codes is one chunk of 16 bytes of a row in the layout of the 128-byte swizzle.  Lanes of
 //                   odd rows write the two halves of the columns in the other order, so that two rows' chunks meet all banks.  (A warp's chunk takes
-//                   1,000 cycles, most of them waits; one team of eight warps: 700 rows, 8,192 x 2,048 were half as fast)
+//                   2,600 cycles, most of them waits; one team of eight warps: 700 rows, 8,192 x 2,048 were half as fast)
 //   warp 0          copies the rows of x (TMA)
 //   warp 1          multiplies (tcgen05.mma, D [128 x rows of x], 32-bit, in TMEM)
 // In the end D goes through shared memory, so that a warp finishes whole rows of results.
-// Bound by the hand-over of stages: of a stage's 1,000 cycles the thread that multiplies waits for its barrier or issues, where the products
-// themselves take 512 (and shared memory's traffic, 32 KB written and read for each chunk, about as much).
+// Bound by the way of a chunk through the SM, some 650 cycles whatever the number of rows of x (33 rows, 18,944 columns: 0.34 us for each 64 columns;
+// 128 rows: 0.38), where the products take 128 and their operands' way in and out of shared memory 420 to 580.  What did not shorten it, at 700 rows,
+// 8,192 x 2,048 (52 us) and 33 rows, 4,096 x 16,384 (31): a second warp that multiplies (53.6, 32.6), 24 decoding warps (57, 34), three stages and two
+// slots (53.3, 32), the scales through shared memory (54.4, 31.2).
 //
 // Where blocks are few, those of a cluster share the columns, and add their sums through distributed shared memory, in their order.
 #include "common.cuh"
@@ -32,7 +34,7 @@ using namespace sm100;
 
 namespace {
 
-constexpr int BM = 128, BN = 128, KC = 64, STAGES = 3, SLOTS = 2, SLOT_CHUNKS = 4;        // a stage holds two chunks
+constexpr int BM = 128, BN = 128, KC = 64, STAGES = 2, SLOTS = 5, SLOT_CHUNKS = 4;        // a stage holds two chunks
 constexpr int TEAMS = SLOT_CHUNKS, TEAM = 4, DECODERS = TEAMS * TEAM, THREADS = (3 + DECODERS) * 32;
 constexpr int A_BYTES = BM * KC * 2, B_BYTES = BN * KC * 2, SLOT_BYTES = 8 * SLOT_CHUNKS * 512, STAGE_BYTES = 2 * (A_BYTES + B_BYTES), SMEM = STAGES * STAGE_BYTES + SLOTS * SLOT_BYTES + 1024;
 constexpr int PITCH = BM + 4;                            // of a row of x's sums, floats
@@ -51,11 +53,11 @@ struct Many {
 // Not inlined: sixteen copies of every activation are more code than a block runs through, and their way to the SM was a third of the kernel's time.
 __device__ __noinline__ float activated(float v, int act) { return apply_activation_wide(v, act); }
 
-// Columns 2 i, 2 i + 1 of a word's eight, times the scale.
-__device__ __forceinline__ uint32_t two_weights(uint32_t word, int i, uint32_t scale) {
-    const uint32_t u = (word >> (4 * i) & 0x000f000fu) | 0x64006400u;
+// Columns 2 i, 2 i + 1 of a word's eight, times the scale: (16 + c) s - 24 s, and 24 s is exact.
+__device__ __forceinline__ uint32_t two_weights(uint32_t word, int i, uint32_t scale, uint32_t less) {
+    const uint32_t u = ((i < 2 ? word << (6 - 4 * i) : word >> (4 * i - 6)) & 0x03c003c0u) | 0x4c004c00u;
     uint32_t w;
-    asm("{ .reg .b32 t; sub.rn.f16x2 t, %1, %2; mul.rn.f16x2 %0, t, %3; }" : "=r"(w) : "r"(u), "r"(0x64086408u), "r"(scale));
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(w) : "r"(u), "r"(scale), "r"(less));
     return w;
 }
 
@@ -128,7 +130,7 @@ q4_units_kernel(__half* __restrict__ xh, float* __restrict__ x_unit, float* __re
 
 template <int GROUP>
 __global__ void __launch_bounds__(THREADS, 1)
-q4_many_kernel(const __grid_constant__ CUtensorMap map_x, const Many p) {
+q4_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_codes, const Many p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     __shared__ uint64_t full[STAGES], empty[STAGES], done, c_full[SLOTS], c_empty[SLOTS];
@@ -143,12 +145,13 @@ q4_many_kernel(const __grid_constant__ CUtensorMap map_x, const Many p) {
     const int c0 = (int)rank * p.share, n = max(0, min(p.share, p.chunks - c0));        // this block's chunks
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < STAGES; ++i) { mbar_init(&full[i], 2 * TEAM * 32 + 1); mbar_init(&empty[i], 1); }
+        for (int i = 0; i < STAGES; ++i) { mbar_init(&full[i], 2 * TEAM + 1); mbar_init(&empty[i], 1); }
         for (int i = 0; i < SLOTS; ++i) { mbar_init(&c_full[i], 1); mbar_init(&c_empty[i], DECODERS); }
         mbar_init(&done, 1);
         aborted = 0;
         mbar_fence_init();
         prefetch_tensormap(&map_x);
+        prefetch_tensormap(&map_codes);
     }
     if (warp == 1) { tmem_alloc(&tmem_slot, BN); tmem_relinquish(); }
     tc_fence_before_sync();
@@ -230,16 +233,21 @@ q4_many_kernel(const __grid_constant__ CUtensorMap map_x, const Many p) {
             if (!ok) { if (lane == 0) atomicExch(p.status, 133); aborted = 1; break; }
             // Half a stage at the end has nothing to write, but its arrival is for this phase too: not before the stage is free, or the stage's last
             // phase, still short of others, would count it.
-            if (i >= n) { mbar_arrive(&full[st]); break; }
+            if (i >= n) {
+                if (lane == 0) mbar_arrive(&full[st]);
+                break;
+            }
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-                uint32_t unit[PER][2];
+                uint32_t unit[PER][2], less[PER][2];
 #pragma unroll
                 for (int h = 0; h < PER; ++h) {
                     const uint32_t two = ahead[turn][h][q];
                     const __half2 a = __float2half2_rn(__uint_as_float(two << 16) * inv[q][0]), b = __float2half2_rn(__uint_as_float(two & 0xffff0000u) * inv[q][1]);
                     unit[h][0] = *reinterpret_cast<const uint32_t*>(&a);
                     unit[h][1] = *reinterpret_cast<const uint32_t*>(&b);
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(less[h][k]) : "r"(unit[h][k]), "r"(0xce00ce00u));       // -24
                 }
                 const uint4 raw = *reinterpret_cast<const uint4*>(slots + slot * SLOT_BYTES + ((mine + q) * SLOT_CHUNKS + i % SLOT_CHUNKS) * 512 + lane * 16);
                 uint8_t* tile = smem + st * STAGE_BYTES + (i & 1) * A_BYTES + (16 * (mine + q) + g) * 128;
@@ -248,14 +256,17 @@ q4_many_kernel(const __grid_constant__ CUtensorMap map_x, const Many p) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const int at = ((4 * ((k >> 1) ^ odd) + t) ^ g) << 4;
-                    const uint32_t s = PER == 1 ? unit[0][k & 1] : (k >> 1) ^ odd ? unit[PER - 1][k & 1] : unit[0][k & 1];
-                    *reinterpret_cast<uint4*>(tile + (k & 1) * 8 * 128 + at) = make_uint4(two_weights(w[k], 0, s), two_weights(w[k], 1, s), two_weights(w[k], 2, s), two_weights(w[k], 3, s));
+                    const bool second = PER == 2 && ((k >> 1) ^ odd);
+                    const uint32_t s = second ? unit[PER - 1][k & 1] : unit[0][k & 1], l = second ? less[PER - 1][k & 1] : less[0][k & 1];
+                    *reinterpret_cast<uint4*>(tile + (k & 1) * 8 * 128 + at) = make_uint4(two_weights(w[k], 0, s, l), two_weights(w[k], 1, s, l), two_weights(w[k], 2, s, l), two_weights(w[k], 3, s, l));
                 }
             }
             fence_proxy_async_smem();
-            mbar_arrive(&full[st]);
             __syncwarp();
-            if (lane == 0) mbar_arrive(&c_empty[slot]);
+            if (lane == 0) {                             // (32 arrivals of a warp would come one behind the other)
+                mbar_arrive(&full[st]);
+                mbar_arrive(&c_empty[slot]);
+            }
             fetch(ahead[turn], i + 2 * TEAMS);
         }
     } else {
@@ -265,14 +276,10 @@ q4_many_kernel(const __grid_constant__ CUtensorMap map_x, const Many p) {
             int i = 0;
             const int count = (n + SLOT_CHUNKS - 1) / SLOT_CHUNKS;
             for (; i < count && !aborted; ++i) {
-                const int slot = i % SLOTS, here = min(SLOT_CHUNKS, n - i * SLOT_CHUNKS);
+                const int slot = i % SLOTS;
                 if (!mbar_wait(&c_empty[slot], ((i / SLOTS) & 1) ^ 1)) { atomicExch(p.status, 136); aborted = 1; break; }
-                mbar_expect_tx(&c_full[slot], 8 * here * 512);
-                for (int k = 0; k < 8; ++k) {            // a tile that is not there: the last one, for nobody
-                    const uint4* src = p.codes + ((size_t)min((row0 >> 4) + k, tiles - 1) * p.chunks + c0 + i * SLOT_CHUNKS) * 32;
-                    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                                 ::"r"(smem_u32(slots + slot * SLOT_BYTES + k * SLOT_CHUNKS * 512)), "l"(src), "r"(here * 512), "r"(smem_u32(&c_full[slot])) : "memory");
-                }
+                mbar_expect_tx(&c_full[slot], SLOT_BYTES);         // (chunks behind the block's and tiles behind the last: read or zeros, for nobody)
+                tma_load_4d(slots + slot * SLOT_BYTES, &map_codes, &c_full[slot], 0, c0 + i * SLOT_CHUNKS, row0 >> 4, 0);
             }
             for (int k = max(0, i - SLOTS); k < i; ++k) mbar_wait(&c_full[k % SLOTS], (k / SLOTS) & 1);       // no copy outlives the block
         }
@@ -378,7 +385,7 @@ EncodeTiledFn encode_fn() {
 }
 
 template <int GROUP>
-int go(const Many& p, const CUtensorMap& map, dim3 grid, int blocks, cudaStream_t stream) {
+int go(const Many& p, const CUtensorMap& map, const CUtensorMap& map_codes, dim3 grid, int blocks, cudaStream_t stream) {
     static PerDevice limit;
     int device = 0;
     cudaGetDevice(&device);
@@ -396,7 +403,7 @@ int go(const Many& p, const CUtensorMap& map, dim3 grid, int blocks, cudaStream_
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, q4_many_kernel<GROUP>, map, p);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, q4_many_kernel<GROUP>, map, map_codes, p);
     if (e != cudaSuccess) return qs_fail(QS_ERR_INTERNAL, "q4 linear: %s", cudaGetErrorString(e));
     return qs_check_launch("q4 linear");
 }
@@ -433,12 +440,19 @@ int q4_linear_many(void* out, int out_dtype, long long ldo, const void* x, long 
     const CUresult rc = fn(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, xh, dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (rc != CUDA_SUCCESS) return qs_fail(QS_ERR_INTERNAL, "q4 linear: cuTensorMapEncodeTiled failed with %d", (int)rc);
+    CUtensorMap map_codes;                               // words, chunks, tiles
+    const cuuint64_t code_dims[4] = {128, (cuuint64_t)chunks, (cuuint64_t)tiles, 1};
+    const cuuint64_t code_strides[3] = {512, (cuuint64_t)chunks * 512, (cuuint64_t)tiles * chunks * 512};
+    const cuuint32_t code_box[4] = {128, SLOT_CHUNKS, 8, 1}, ones[4] = {1, 1, 1, 1};
+    const CUresult rc2 = fn(&map_codes, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, const_cast<void*>(codes), code_dims, code_strides, code_box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (rc2 != CUDA_SUCCESS) return qs_fail(QS_ERR_INTERNAL, "q4 linear: cuTensorMapEncodeTiled failed with %d", (int)rc2);
     const int o = out_dtype == QS_F32 ? 16 : 8;
     const int vector = ((uintptr_t)out % o) == 0 && ldo % 4 == 0 && ldr % 4 == 0 && ((uintptr_t)res0 % 8) == 0 && ((uintptr_t)res1 % 8) == 0;
     const Many p = {out, row_unit, x_unit, bias, res0, res1, (const uint4*)codes, (const uint32_t*)scales, (size_t)ldo, (size_t)ldr, M, N, chunks, (chunks + blocks - 1) / blocks, columns,
                     out_dtype, bias_dtype, act, settled, vector, status};
     const dim3 grid(row_tiles * blocks, column_tiles);
-    if (group == 32) return go<32>(p, map, grid, blocks, stream);
-    if (group == 64) return go<64>(p, map, grid, blocks, stream);
-    return go<128>(p, map, grid, blocks, stream);
+    if (group == 32) return go<32>(p, map, map_codes, grid, blocks, stream);
+    if (group == 64) return go<64>(p, map, map_codes, grid, blocks, stream);
+    return go<128>(p, map, map_codes, grid, blocks, stream);
 }
