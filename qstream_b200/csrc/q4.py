@@ -42,12 +42,14 @@ class Weight4:
     codes: uint8 [ceil(out / 16)][ceil(in / 64)][32][16].  Entry 4 g + t of a tile is four little-endian words of eight codes; word
     2 h + u holds row g + 8 u of the tile, columns 32 h + 8 t + (0, 2, 4, 6, 1, 3, 5, 7), lowest four bits first.
     scales: bfloat16 [ceil(out / 16)][groups][8][2], entry (g, u) for row g + 8 u; groups cover the columns rounded up to 64.
-    What fills up the last rows and columns are codes of 8 and scales of 0."""
-    __slots__ = ("codes", "scales", "out_features", "in_features", "group", "_at")
+    What fills up the last rows and columns are codes of 8 and scales of 0.
+    The two tensors are checked once, here, so they stay: their contents may change, another tensor takes another matrix."""
+    __slots__ = ("codes", "scales", "out_features", "in_features", "group")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, out_features: int, in_features: int, group: int):
-        n, k, g = self.out_features, self.in_features, self.group = out_features, in_features, group
-        self.codes, self.scales = codes, scales
+        n, k, g = out_features, in_features, group
+        for name, value in zip(self.__slots__, (codes, scales, n, k, g)):
+            object.__setattr__(self, name, value)
         if n < 1 or k < 1 or g not in GROUPS:
             _refuse(f"4-bit weights: a matrix [{n}, {k}] in groups of {g} (groups: {GROUPS})", QsError.QUANT_MISMATCH)
         tiles, chunks = -(-n // 16), -(-k // 64)
@@ -55,10 +57,14 @@ class Weight4:
                 or scales.shape != (tiles, -(-chunks * 64 // g), 8, 2) or scales.dtype is not torch.bfloat16 or not scales.is_contiguous():
             _refuse(f"4-bit weights: [{n}, {k}] in groups of {g} are contiguous uint8 codes and bfloat16 scales of {sizes(n, k, g)}, got {codes.dtype} "
                     f"{tuple(codes.shape)} and {scales.dtype} {tuple(scales.shape)}", QsError.QUANT_MISMATCH)
-        # (device, addresses) for the calls
-        self._at = codes.get_device(), codes.data_ptr(), scales.data_ptr()
-        if scales.get_device() != self._at[0] or self._at[1] % 16 or self._at[2] % 4:
+        if scales.get_device() != codes.get_device() or codes.data_ptr() % 16 or scales.data_ptr() % 4:
             _refuse("4-bit weights: codes and scales lie on one device, the codes on a 16-byte boundary")
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"a 4-bit matrix keeps its {name}")
+
+    def __reduce__(self):
+        return Weight4, (self.codes, self.scales, self.out_features, self.in_features, self.group)
 
     @property
     def shape(self):
@@ -140,8 +146,8 @@ def linear(x, weight: Weight4, bias=None, activation=None, residuals=(), out_dty
         out, r0, r1, ldr = torch.empty((M, N), dtype=want, device=x.device), None, None, N
     if M == 0:
         return out
-    device, codes, scales = weight._at
-    stream = launch_stream(device, x, bias, out, r0, r1)
+    codes, scales = weight.codes, weight.scales
+    stream = launch_stream(codes.get_device(), x, bias, out, r0, r1)
     if _linear is None:
         _bind()
     code, at = (ops.F32, x.data_ptr()) if wide else (ops.BF16, x.data_ptr())
@@ -152,7 +158,7 @@ def linear(x, weight: Weight4, bias=None, activation=None, residuals=(), out_dty
         if nbytes:
             scratch = torch.empty((nbytes,), dtype=torch.uint8, device=x.device)
             ops.count_launches(_kernels(M, N, K, code, aligned) - 1)
-    ops.check(_linear(out.data_ptr(), ops.F32 if want is torch.float32 else ops.BF16, out.stride(0), at, code, ldx, aligned, codes, scales,
+    ops.check(_linear(out.data_ptr(), ops.F32 if want is torch.float32 else ops.BF16, out.stride(0), at, code, ldx, aligned, codes.data_ptr(), scales.data_ptr(),
                       None if bias is None else bias.data_ptr(), 0 if bias is None else ops.dtype_code(bias), act, None if r0 is None else r0.data_ptr(),
                       None if r1 is None else r1.data_ptr(), ldr, M, N, K, weight.group, 1 if settled else 0, None if scratch is None else scratch.data_ptr(),
                       gemm_tc.status_word(x.device).data_ptr(), stream))

@@ -1,4 +1,6 @@
 """Matrix products with 4-bit weights (csrc/q4.cu) against float64."""
+import copy
+
 import numpy as np
 import pytest
 import torch
@@ -161,6 +163,17 @@ def test_a_float32_row_is_the_same_bits_in_any_batch():
         whole = q4.linear(x, w)
         for m in (1, 2, 3, 5, 6, 16, 33):
             assert torch.equal(q4.linear(x[:m], w), whole[:m])
+
+
+def test_a_matrix_that_moves_is_read_where_it_lies():
+    w = q4.quantize(normal(6, 90, 700, std=0.1), 64)
+    twin = copy.deepcopy(w)
+    x = normal(7, 3, 700)
+    want = q4.linear(x, w)
+    w.codes.data, w.scales.data = w.codes.data.clone(), w.scales.data.clone()
+    assert torch.equal(q4.linear(x, w), want) and torch.equal(q4.linear(x, twin), want)
+    w.codes.copy_(torch.full_like(w.codes, 0x88))
+    assert (q4.linear(x, w) == 0).all() and torch.equal(q4.linear(x, twin), want)
 
 
 @pytest.mark.parametrize("n,k", [(70, 16500), (33, 32768), (20, 9000)])

@@ -1,4 +1,6 @@
 """What the calls over 4-bit weights and 8-bit pages refuse, before anything reaches a device."""
+import copy
+
 import pytest
 import torch
 
@@ -15,6 +17,15 @@ def refused(code, call, *args, **kw):
     with pytest.raises(QStreamError) as e:
         call(*args, **kw)
     assert e.value.code == code, e.value
+
+
+def test_a_packed_matrix_keeps_what_was_checked():
+    w = weight()
+    for name, value in (("codes", w.codes.clone()), ("scales", w.scales.clone()), ("out_features", 48), ("in_features", 128), ("group", 64), ("other", 1)):
+        with pytest.raises(AttributeError):
+            setattr(w, name, value)
+    twin = copy.deepcopy(w)
+    assert twin.shape == w.shape and twin.group == w.group and twin.codes.data_ptr() != w.codes.data_ptr() and torch.equal(twin.codes, w.codes)
 
 
 def test_packed_matrices_that_do_not_fit():
