@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import functools
 from ctypes import c_int, c_longlong, c_void_p
+from operator import attrgetter
 
 import torch
 
@@ -44,12 +45,12 @@ class Weight4:
     scales: bfloat16 [ceil(out / 16)][groups][8][2], entry (g, u) for row g + 8 u; groups cover the columns rounded up to 64.
     What fills up the last rows and columns are codes of 8 and scales of 0.
     The two tensors are checked once, here, so they stay: their contents may change, another tensor takes another matrix."""
-    __slots__ = ("codes", "scales", "out_features", "in_features", "group")
+    __slots__ = ("_codes", "_scales", "_n", "_k", "_group")
+    codes, scales, out_features, in_features, group = (property(attrgetter(name)) for name in __slots__)
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, out_features: int, in_features: int, group: int):
-        n, k, g = out_features, in_features, group
-        for name, value in zip(self.__slots__, (codes, scales, n, k, g)):
-            object.__setattr__(self, name, value)
+        n, k, g = self._n, self._k, self._group = out_features, in_features, group
+        self._codes, self._scales = codes, scales
         if n < 1 or k < 1 or g not in GROUPS:
             _refuse(f"4-bit weights: a matrix [{n}, {k}] in groups of {g} (groups: {GROUPS})", QsError.QUANT_MISMATCH)
         tiles, chunks = -(-n // 16), -(-k // 64)
@@ -59,9 +60,6 @@ class Weight4:
                     f"{tuple(codes.shape)} and {scales.dtype} {tuple(scales.shape)}", QsError.QUANT_MISMATCH)
         if scales.get_device() != codes.get_device() or codes.data_ptr() % 16 or scales.data_ptr() % 4:
             _refuse("4-bit weights: codes and scales lie on one device, the codes on a 16-byte boundary")
-
-    def __setattr__(self, name, value):
-        raise AttributeError(f"a 4-bit matrix keeps its {name}")
 
     def __reduce__(self):
         return Weight4, (self.codes, self.scales, self.out_features, self.in_features, self.group)
@@ -146,7 +144,7 @@ def linear(x, weight: Weight4, bias=None, activation=None, residuals=(), out_dty
         out, r0, r1, ldr = torch.empty((M, N), dtype=want, device=x.device), None, None, N
     if M == 0:
         return out
-    codes, scales = weight.codes, weight.scales
+    codes, scales = weight._codes, weight._scales
     stream = launch_stream(codes.get_device(), x, bias, out, r0, r1)
     if _linear is None:
         _bind()
