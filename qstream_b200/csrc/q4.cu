@@ -91,7 +91,14 @@ q4_quantize_kernel(uint32_t* __restrict__ codes, __nv_bfloat16* __restrict__ sca
 //
 // WARPS warps of a block share a tile's columns, the blocks of a cluster share them again where there are more than they hold or tiles are few; a
 // block's sums go through shared memory, a cluster's through distributed shared memory, in a fixed order.
-constexpr int WARPS = 16, TILES = 8;
+//
+// A block sums up a round of tiles at a time: eight, or as many as its teams of warps take with the AHEAD tiles that each has on its way.  A round is
+// a multiple of those: a tile's place among the ones on their way is its turn modulo AHEAD, and the next round begins with place 0 again.
+constexpr int WARPS = 16, TILES = 8, AHEAD = 2;
+constexpr int round_of(int share) {
+    const int turns = AHEAD * (WARPS / share);
+    return turns > TILES ? turns : TILES / turns * turns;
+}
 template <int NT> constexpr int own_chunks() { return 4 / NT; }
 template <int NT> constexpr int warp_sums() { return NT * 8 * 17; }
 
@@ -145,16 +152,16 @@ struct Few {
     const uint4* codes;
     const uint32_t* scales;
     size_t ldo, ldx, ldr;
-    int M, N, chunks, share, terms, out_dtype, res_dtype, bias_dtype, act, settled;
+    int M, N, chunks, share, round, terms, out_dtype, res_dtype, bias_dtype, act, settled;
 };
 
 template <int NT, int GROUP>
 __global__ void __launch_bounds__(WARPS * 32, 1)
 q4_few_kernel(const Few p) {
-    // COLS columns of x; a warp's OWN chunks of columns, whose part of x it keeps in registers; tiles AHEAD on their way
-    constexpr int COLS = NT * 8, OWN = own_chunks<NT>(), AHEAD = 2, SUMS = warp_sums<NT>();
+    // COLS columns of x; a warp's OWN chunks of columns, whose part of x it keeps in registers
+    constexpr int COLS = NT * 8, OWN = own_chunks<NT>(), SUMS = warp_sums<NT>();
     constexpr int SCALES = GROUP == 32 ? 2 * OWN : GROUP == 64 ? OWN : OWN / 2;
-    extern __shared__ __align__(16) float part[];        // [TILES][warps that share a tile's columns][COLS][17]
+    extern __shared__ __align__(16) float part[];        // [tiles of a round][warps that share a tile's columns][COLS][17]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     uint32_t rank, blocks;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
@@ -162,7 +169,7 @@ q4_few_kernel(const Few p) {
     const int chunks = p.chunks, groups = (chunks * 64 + GROUP - 1) / GROUP, tokens = COLS / p.terms, m0 = blockIdx.y * tokens;
     const int tiles = (p.N + 15) >> 4, cluster = blockIdx.x / blocks, n_clusters = gridDim.x / blocks;
     // the warps: `share` of them share a tile's columns, `teams` of these take tiles in turn
-    const int share = p.share, teams = WARPS / share, team = warp / share, c0 = ((int)rank * share + warp % share) * OWN;
+    const int share = p.share, teams = WARPS / share, round = p.round, team = warp / share, c0 = ((int)rank * share + warp % share) * OWN;
     const int n = team < teams ? max(0, min(OWN, chunks - c0)) : 0;          // this warp's chunks
     const int n_tiles = cluster < tiles ? (tiles - 1 - cluster) / n_clusters + 1 : 0;   // of the cluster: cluster, + n_clusters, ...
 
@@ -207,12 +214,12 @@ q4_few_kernel(const Few p) {
     for (int i = 0; i < AHEAD; ++i) load(b[i], team + i * teams);
     if (p.settled) load_rows();
     const uint32_t base = sm100::smem_u32(part);
-    for (int first = 0; first < n_tiles; first += TILES) {
-        for (int k0 = first + team; k0 < min(first + TILES, n_tiles); k0 += AHEAD * teams) {
+    for (int first = 0; first < n_tiles; first += round) {
+        for (int k0 = first + team; k0 < min(first + round, n_tiles); k0 += AHEAD * teams) {
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) {
                 const int k = k0 + i * teams;
-                if (k >= min(first + TILES, n_tiles) || n == 0) break;
+                if (k >= min(first + round, n_tiles) || n == 0) break;
                 float acc[NT][4];
 #pragma unroll
                 for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
@@ -252,8 +259,8 @@ q4_few_kernel(const Few p) {
                     for (int e = 0; e < 4; ++e) to[(8 * j + 2 * t + (e & 1)) * 17 + g + 8 * (e >> 1)] = acc[j][e];
             }
         }
-        const int some = min(TILES, n_tiles - first), parts = (min(p.chunks - (int)rank * share * OWN, share * OWN) + OWN - 1) / OWN;
-        if (first + TILES >= n_tiles) grid_dep_launch();
+        const int some = min(round, n_tiles - first), parts = (min(p.chunks - (int)rank * share * OWN, share * OWN) + OWN - 1) / OWN;
+        if (first + round >= n_tiles) grid_dep_launch();
         __syncthreads();
         auto block_sum = [&](int k, int at) {            // over the warps, in their order
             const float* from = part + k * share * SUMS + at;
@@ -310,7 +317,8 @@ int few_launch(Few p, cudaStream_t stream) {
     while (blocks < 8 && (p.chunks > blocks * WARPS * OWN || (p.chunks >= 8 * blocks * OWN && tiles * blocks * 2 <= 148))) blocks *= 2;
     QS_REQUIRE(p.chunks <= blocks * WARPS * OWN, "q4 linear: %d columns exceed what the blocks of a cluster hold (%d)", p.chunks * 64, 8 * WARPS * OWN * 64);
     p.share = ((p.chunks + blocks - 1) / blocks + OWN - 1) / OWN;
-    const int smem = TILES * p.share * warp_sums<NT>() * 4;
+    p.round = round_of(p.share);
+    const int smem = p.round * p.share * warp_sums<NT>() * 4;       // of TILES * WARPS sums at most: AHEAD * WARPS where a round is longer than TILES
     static PerDevice limit, room[4];
     int device = 0;
     cudaGetDevice(&device);
@@ -387,7 +395,7 @@ QS_API int qs_q4_linear(void* out, int out_dtype, long long ldo, const void* x, 
     const int e = dtype == QS_F32 ? 4 : 2, chunks = (K + 63) / 64;
     QS_REQUIRE(!aligned || (((uintptr_t)x % 16) == 0 && ldx * e % 16 == 0), "q4 linear: rows off their 16-byte boundaries");
     Few p = {out, (const __nv_bfloat16*)x, bias, res0, res1, (const uint4*)codes, (const uint32_t*)scales, (size_t)ldo, (size_t)ldx, (size_t)ldr,
-             M, N, chunks, 0, dtype == QS_F32 ? 3 : 1, out_dtype, dtype, bias_dtype, act, settled};
+             M, N, chunks, 0, 0, dtype == QS_F32 ? 3 : 1, out_dtype, dtype, bias_dtype, act, settled};
     const long long rows = rows_scratch(M, K, dtype, aligned);
     if (rows > 0) {
         QS_REQUIRE(scratch && ((uintptr_t)scratch % 16) == 0, "q4 linear: no workspace");
