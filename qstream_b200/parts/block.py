@@ -405,7 +405,8 @@ class ScaledParallelBlock(Arrangement):
         self.wide = torch.float32
         self._typed = {id(p): "out_dtype" in inspect.signature(p.forward).parameters for p in (self.mixer, self.ffn) if p}
         self.fused_weight = None
-        if self.ffn is None or runtime.dtype != torch.bfloat16 or getattr(self.mixer.spec, "gate", False) \
+        # (matrices in 4 bits stay apart, as in ParallelBlock)
+        if self.ffn is None or runtime.weight_group or runtime.dtype != torch.bfloat16 or getattr(self.mixer.spec, "gate", False) \
                 or not all(hasattr(p, "output_projection") and hasattr(p, "forward_hidden") for p in (self.mixer, self.ffn)):
             return
         (wm, bm), (wf, bf) = self.mixer.output_projection(), self.ffn.output_projection()

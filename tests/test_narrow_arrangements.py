@@ -1,0 +1,35 @@
+"""Every small model whose layers hold a matrix of attention or of a dense feed-forward loads with 4-bit weights, in both types (the rounding
+itself needs a GPU and is left out here)."""
+import importlib
+
+import pytest
+import torch
+
+import qstream_b200 as qs
+from qstream_b200.csrc import q4
+from qstream_b200.errors import QsError, QStreamError
+
+MODELS = [(name, which) for name in ("lutelorn", "fofinex", "sefuvik", "nutatar", "fotanex", "vofinex") for which in sorted(importlib.import_module(name + "_util").CONFIGS)]
+# models of mixers and experts alone, whose matrices stay as they are stored
+WIDE_ONLY = {("fofinex", "L"), ("sefuvik", "R"), ("nutatar", "G"), ("nutatar", "L"), ("nutatar", "M"), ("fotanex", "R"), ("fotanex", "S"), ("fotanex", "M")}
+
+
+def rounded(weight, group=64):
+    n, k = weight.shape
+    codes, scales = q4.sizes(n, k, group)
+    return q4.Weight4(torch.full(codes, 0x88, dtype=torch.uint8), torch.zeros(scales, dtype=torch.bfloat16), n, k, group)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("name,which", MODELS)
+def test_every_arrangement_takes_narrow_matrices(tmp_path, monkeypatch, name, which, dtype):
+    monkeypatch.setattr(q4, "quantize", rounded)
+    folder, _ = importlib.import_module(name + "_util").make_folder(tmp_path, which, dtype)
+    load = lambda **kw: qs.load_model(folder, dtype=dtype, device="cpu", allow_mmap=False, **kw)       # noqa: E731
+    if (name, which) in WIDE_ONLY:
+        with pytest.raises(QStreamError) as e:
+            load(weight_bits=4)
+        assert e.value.code == QsError.UNSUPPORTED_ARCH
+        return
+    wide, narrow = load(), load(weight_bits=4, weight_group=32)
+    assert narrow.runtime.narrowed and narrow.n_parameters == wide.n_parameters and narrow.weight_bytes < wide.weight_bytes
