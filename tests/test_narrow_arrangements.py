@@ -33,3 +33,13 @@ def test_every_arrangement_takes_narrow_matrices(tmp_path, monkeypatch, name, wh
         return
     wide, narrow = load(), load(weight_bits=4, weight_group=32)
     assert narrow.runtime.narrowed and narrow.n_parameters == wide.n_parameters and narrow.weight_bytes < wide.weight_bytes
+
+
+def test_what_a_key_takes_does_not_depend_on_how_the_matrices_are_held(tmp_path, monkeypatch):
+    from util import make_folder
+    monkeypatch.setattr(q4, "quantize", rounded)
+    for dtype, size in (("float32", 4), ("bfloat16", 2)):
+        folder, _ = make_folder(tmp_path, "A", dtype)
+        for bits in (None, 4):
+            mixer = qs.load_model(folder, dtype=dtype, device="cpu", allow_mmap=False, weight_bits=bits).blocks[0].mixer
+            assert mixer.cache_bytes_per_key == size * mixer.spec.n_kv_heads * (mixer.spec.head_dim + mixer.spec.value_dim)
