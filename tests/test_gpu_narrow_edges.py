@@ -1,0 +1,65 @@
+"""The operators over 4-bit weights and 8-bit pages at the ends of their ranges."""
+import numpy as np
+import pytest
+import torch
+
+import narrow_util as U
+from qstream_b200.csrc import kv8, q4
+
+pytestmark = pytest.mark.gpu
+TYPES = {"bf16": torch.bfloat16, "f32": torch.float32}
+
+
+def i32(x):
+    return torch.as_tensor(np.asarray(x), dtype=torch.int32).cuda()
+
+
+def device(pages):
+    return [torch.from_numpy(x).cuda() for x in pages[:4]], i32(pages[4])
+
+
+def normal(seed, *shape, std=1.0, dtype=torch.float32):
+    return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * std).to(dtype).cuda()
+
+
+def close(got, want, bound, what=None):
+    err = np.abs(U.f64(got).reshape(want.shape) - want)
+    assert (err <= bound).all(), (what, float(np.nanmax(err / np.maximum(bound, 1e-300))))
+
+
+class Scaled:
+    """Keys of 2^e against queries of 2^-e, beside values of as much (as far as 150 of them have a sum): what attention makes of pages is what they read back as."""
+
+    def __init__(self, e, size, dtype):
+        rng = np.random.default_rng(size + 200 + e)
+        self.size, self.dtype, self.e_v = size, dtype, min(max(e, -100), 112)
+        kc, vc, ks, vs, table = U.paged(rng, [150, 64], 2, size, size)
+        self.pages = kc, vc, np.full_like(ks, 2.0 ** e), np.full_like(vs, 2.0 ** self.e_v), table
+        self.slot, self.pos = [0] * 20 + [1], list(range(130, 150)) + [63]
+        self.q = (torch.tensor(rng.normal(size=(21, 4 * size))) * 2.0 ** (-e - 6)).to(TYPES[dtype]).cuda()
+        self.status = torch.zeros(1, dtype=torch.int32, device="cuda")
+
+    def run(self, call, rounding=0.0, **rows):
+        dev, table = device(self.pages)
+        got = call(self.q, 4, 2, self.size, self.size ** -0.5, 0, **rows, page_table=table, page_tokens=64, k_cache=dev[0], v_cache=dev[1], k_scale=dev[2], v_scale=dev[3],
+                   status=self.status)
+        want, bound = U.attention(U.f64(self.q).reshape(21, 4, self.size), self.pages[:2], self.pages[2:4], self.slot, self.pos, self.pages[4], 2, self.size ** -0.5,
+                                  wide_weights=self.dtype == "f32", out_bf16=self.dtype == "bf16")
+        close(got, want, bound + rounding * 127 * 2.0 ** self.e_v)
+        assert int(self.status.item()) == 0
+
+    def prompts(self):
+        # weights rounded to bfloat16 on the tensor cores' path: each of them by half a step, 2^-9 of it, at most
+        self.run(kv8.prefill, 2.0 ** -9 if self.dtype == "bf16" and self.size % 16 == 0 else 0.0, tiles=i32([(0, 20, 130, 0), (20, 1, 63, 1)]))
+
+    def single_tokens(self):
+        self.run(kv8.decode, tok_slot=i32(self.slot), tok_pos=i32(self.pos), max_context=150)
+
+
+EXPONENTS = [-126, -110, 0, 90, 100, 104, 105, 112, 120]
+
+
+@pytest.mark.parametrize("size", [64, 80, 144])
+@pytest.mark.parametrize("e", EXPONENTS)
+def test_prompts_over_scales_of_any_size(e, size):
+    Scaled(e, size, "bf16").prompts()
