@@ -336,7 +336,18 @@ kv8_decode_kernel(const DecodeArgs p) {
             s_l[warp][h0 + j] = l[j] * f[j];
             if (warp == 0) s_unit[h0 + j] = M;
         }
-        f[j] *= vs;
+    }
+    // The sums as 2^-15 of what the weights made them (the merge multiplies by as much): with the 2^15, values from 2^90 or so on would have no sum in
+    // 32 bits.  Of very small values the sums are brought down by themselves: f times as little would lose bits.
+    const float unit_v = vs * 0x1p-15f;
+    if (vs < 0x1p-60f) {
+#pragma unroll
+        for (int j = 0; j < VB * 8; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[j][e] *= unit_v;
+    } else {
+        f[0] *= unit_v;
+        f[1] *= unit_v;
     }
 #pragma unroll
     for (int j = 0; j < VB * 8; ++j) {
@@ -375,7 +386,7 @@ kv8_decode_kernel(const DecodeArgs p) {
                 factor = M == -INFINITY ? 1.f : exp2f(M - all);
                 L = fmaf(L, factor, exp2f(sink - all + 15.f));
             }
-            factor *= L != 0.f ? 1.0f / L : 0.f;
+            factor *= L != 0.f ? 0x1p15f / L : 0.f;
             const size_t to = (size_t)row * p.ldo + (size_t)(head0 + h) * dv + d;
             const int type = p.out_f32 ? QS_F32 : QS_BF16;
             store_places(p.out, type, to, o, factor, d + 16 < dv);
@@ -429,7 +440,7 @@ kv8_merge_kernel(const DecodeArgs p) {
         if (seen(u)) weigh(u, p.ml[cell + u]);
     L = block_sum(L, scratch);                           // (a barrier: the weights are there)
     if (p.sink) L += exp2f(sink - M + 15.f);
-    const float inv = L != 0.f ? 1.0f / L : 0.f;
+    const float inv = L != 0.f ? 0x1p15f / L : 0.f;
     constexpr int width = PLACES / 4, groups = MERGE_THREADS / width;
     const int group = threadIdx.x / width, place = threadIdx.x % width * 4, d = dim_of(place);
     const int share = (n + groups - 1) / groups, from = group * share, end = d < dv ? min(n, from + share) : from;

@@ -63,3 +63,10 @@ EXPONENTS = [-126, -110, 0, 90, 100, 104, 105, 112, 120]
 @pytest.mark.parametrize("e", EXPONENTS)
 def test_prompts_over_scales_of_any_size(e, size):
     Scaled(e, size, "bf16").prompts()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", [64, 80, 144])
+@pytest.mark.parametrize("e", EXPONENTS)
+def test_single_tokens_over_scales_of_any_size(e, size, dtype):
+    Scaled(e, size, dtype).single_tokens()
