@@ -369,8 +369,15 @@ kv8_attention_kernel(TO* __restrict__ out, const T* __restrict__ q, const Attend
         for (int d = lane; d < p.dv; d += 32) o[d] = from_f32<TO>(0.f);
         return;
     }
+    // The query over the power of two at or below its largest number: a sum of its products with codes has a place in 32 bits then, however large the query and
+    // small the page's scale.  Numbers that are not finite go through as they are.
     float* qs = q_smem + warp * p.dk;
-    for (int d = lane; d < p.dk; d += 32) qs[d] = to_f32(q[(size_t)row * p.ldq + (size_t)head * p.dk + d]);
+    const T* src = q + (size_t)row * p.ldq + (size_t)head * p.dk;
+    float most = 0.f;
+    for (int d = lane; d < p.dk; d += 32) most = fmaxf(most, fabsf(to_f32(src[d])));
+    const uint32_t e = min(max(__float_as_uint(warp_max(most)) >> 23, 1u), 253u);
+    const float unit = __uint_as_float(e << 23), inverse = __uint_as_float((254u - e) << 23);
+    for (int d = lane; d < p.dk; d += 32) qs[d] = to_f32(src[d]) * inverse;
     __syncwarp();
     const int first = p.chunk > 0 ? pos - pos % p.chunk : p.window > 0 ? max(0, pos - p.window + 1) : 0;
     const int keep = p.window > 0 ? min(p.keep_first, first) : 0;
@@ -392,7 +399,7 @@ kv8_attention_kernel(TO* __restrict__ out, const T* __restrict__ q, const Attend
             const int8_t* kr = p.k_cache + (at * PAGE + (key & 63)) * p.dk;
             float dot = 0.f;
             for (int d = 0; d < p.dk; ++d) dot = fmaf(qs[d], (float)kr[d], dot);
-            s = dot * p.k_scale[at] * p.scale;
+            s = dot * (unit * p.k_scale[at]) * p.scale;
             if (p.softcap > 0.f) s = p.softcap * tanhf(s / p.softcap);
         }
         const float m_new = fmaxf(m, warp_max(s));

@@ -70,3 +70,13 @@ def test_prompts_over_scales_of_any_size(e, size):
 @pytest.mark.parametrize("e", EXPONENTS)
 def test_single_tokens_over_scales_of_any_size(e, size, dtype):
     Scaled(e, size, dtype).single_tokens()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("e", EXPONENTS)
+def test_the_plain_kernel_over_scales_of_any_size(e, dtype):
+    """Head sizes that are no multiples of 16, and prompts of float32 rows."""
+    Scaled(e, 20, dtype).prompts()
+    Scaled(e, 20, dtype).single_tokens()
+    if dtype == "f32":
+        Scaled(e, 64, dtype).prompts()
