@@ -378,18 +378,17 @@ kv8_decode_kernel(const DecodeArgs p) {
             const size_t cell = ((size_t)row * p.n_heads + head0 + h) * p.splits + split;
             *reinterpret_cast<float4*>(p.partial + cell * PLACES + place) = o;
             if (place == 0) p.ml[cell] = make_float2(s_unit[h], L);
-        } else {                                         // as the merge of one split
+        } else {                                         // as the merge of one split: the same roundings, one by one
             const float M = s_unit[h];
-            float factor = 1.f;
             if (p.sink) {
-                const float sink = p.sink[head0 + h] * 1.4426950408889634f, all = fmaxf(M, sink);
-                factor = M == -INFINITY ? 1.f : exp2f(M - all);
-                L = fmaf(L, factor, exp2f(sink - all + 15.f));
+                const float sink = p.sink[head0 + h] * 1.4426950408889634f, all = fmaxf(M, sink), w = M == -INFINITY ? 1.f : exp2f(M - all);
+                L = __fadd_rn(__fmul_rn(L, w), exp2f(sink - all + 15.f));
+                o.x = __fmul_rn(o.x, w); o.y = __fmul_rn(o.y, w); o.z = __fmul_rn(o.z, w); o.w = __fmul_rn(o.w, w);
             }
-            factor *= L != 0.f ? 0x1p15f / L : 0.f;
+            const float inv = L != 0.f ? 0x1p15f / L : 0.f;
             const size_t to = (size_t)row * p.ldo + (size_t)(head0 + h) * dv + d;
             const int type = p.out_f32 ? QS_F32 : QS_BF16;
-            store_places(p.out, type, to, o, factor, d + 16 < dv);
+            store_places(p.out, type, to, o, inv, d + 16 < dv);
         }
     }
 }

@@ -80,3 +80,26 @@ def test_the_plain_kernel_over_scales_of_any_size(e, dtype):
     Scaled(e, 20, dtype).single_tokens()
     if dtype == "f32":
         Scaled(e, 64, dtype).prompts()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", [64, 128, 256])
+def test_a_row_with_a_sink_does_not_depend_on_its_batch(size, dtype):
+    """Contexts of one split, whose results need no merge, and of several: the same bits, whatever the sink counts beside the keys."""
+    rng = np.random.default_rng(21)
+    lens = [1000, 3, 64, 90, 128, 37]
+    pages = U.paged(rng, lens, 2, size, size)
+    dev, table = device(pages)
+    q = torch.tensor(rng.normal(size=(6, 8 * size))).to(TYPES[dtype]).cuda()
+    sink = torch.linspace(-3, 9, 8, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+
+    def run(rows, reach, **kw):
+        return kv8.decode(q[rows], 8, 2, size, size ** -0.5, 0, i32(rows), i32([lens[r] - 1 for r in rows]), table, 64, *dev, reach, status, sink=sink, **kw)
+
+    for out_dtype in (None, torch.float32):
+        whole = run(list(range(6)), 1000, out_dtype=out_dtype)
+        for r in range(1, 6):
+            for reach in (lens[r], 128, 256, 300):
+                assert torch.equal(run([r], reach, out_dtype=out_dtype)[0], whole[r]), (r, reach)
+    assert int(status.item()) == 0
