@@ -41,7 +41,7 @@ struct DecodeArgs {
     const float *k_scale, *v_scale, *sink;
     const int32_t *tok_slot, *tok_pos, *page_table;
     size_t ldo, ldq;
-    int max_pages, n_slots, n_pages, n_heads, n_kv_heads, dk, dv, window, chunk, keep_first, splits, out_f32;
+    int max_pages, n_slots, n_pages, n_heads, n_kv_heads, dk, dv, window, chunk, keep_first, splits, reach, out_f32;
     float scale, softcap, cap_k2;
     int q_aligned;
     int32_t* status;
@@ -142,7 +142,7 @@ kv8_decode_kernel(const DecodeArgs p) {
             for (int i = 0; i < 8; ++i) x[c][i] = 8 * lane + i < dk ? to_f32(src[i]) : 0.f;
         }
     }
-    if (slot < 0 || slot >= p.n_slots || pos < 0 || (pos >> 6) >= p.max_pages || pos >= p.splits * SPLIT) {
+    if (slot < 0 || slot >= p.n_slots || pos < 0 || (pos >> 6) >= p.max_pages || pos >= p.reach) {
         if (slot >= 0 && threadIdx.x == 0 && split == 0 && blockIdx.y == 0) atomicExch(p.status, 1);
         if (p.splits == 1)                               // no merge: the row's zeros are written here
             for (int i = threadIdx.x; i < heads * dv; i += WARPS * 32) store_from_f32(p.out, p.out_f32 ? QS_F32 : QS_BF16, (size_t)row * p.ldo + (size_t)head0 * dv + i, 0.f);
@@ -411,7 +411,7 @@ kv8_merge_kernel(const DecodeArgs p) {
     float2 ml = make_float2(0.f, 0.f);
     if ((int)threadIdx.x < p.splits) asm volatile("ld.global.v2.f32 {%0, %1}, [%2];" : "=f"(ml.x), "=f"(ml.y) : "l"(p.ml + cell + threadIdx.x));
     const float sink = p.sink ? p.sink[head] * 1.4426950408889634f : -INFINITY;
-    if (slot < 0 || slot >= p.n_slots || pos < 0 || (pos >> 6) >= p.max_pages || pos >= p.splits * SPLIT) {       // padding, or reported: a defined row
+    if (slot < 0 || slot >= p.n_slots || pos < 0 || (pos >> 6) >= p.max_pages || pos >= p.reach) {       // padding, or reported: a defined row
         for (int d = threadIdx.x; d < dv; d += MERGE_THREADS) store_from_f32(p.out, type, to + d, 0.f);
         return;
     }
@@ -503,7 +503,7 @@ QS_API long long qs_kv8_decode_scratch(int T_tokens, int n_heads, int dk, int dv
 
 // out [T, n_heads * dv] (bfloat16, or float32 with out_f32), q [T, n_heads * dk] of type `dtype`; head sizes multiples of 16 up to 256.  `partial`: float32,
 // qs_kv8_decode_scratch elements, 16-byte aligned; contents need no initialisation; may be null for one split.
-// Masks, status codes and rows as for qs_kv8_attention; positions lie below max_context rounded up to whole splits.
+// Masks, status codes and rows as for qs_kv8_attention; positions lie below max_context.
 QS_API int qs_kv8_decode(void* out, int out_f32, long long ldo, const void* q, int dtype, long long ldq, int T_tokens, const int32_t* tok_slot,
                          const int32_t* tok_pos, const int32_t* page_table, int n_slots, int max_pages, int n_pages, const int8_t* k_cache,
                          const int8_t* v_cache, const float* k_scale, const float* v_scale, int n_heads, int n_kv_heads, int dk, int dv, float scale,
@@ -523,7 +523,7 @@ QS_API int qs_kv8_decode(void* out, int out_f32, long long ldo, const void* q, i
     const int e = dtype == QS_F32 ? 4 : 2;
     const int q_aligned = ((uintptr_t)q % 16) == 0 && ldq * e % 16 == 0;
     const DecodeArgs p = {out, partial, (float2*)(partial + (size_t)T_tokens * n_heads * splits * places(dk, dv)), q, k_cache, v_cache, k_scale, v_scale, sink, tok_slot, tok_pos, page_table, (size_t)ldo, (size_t)ldq,
-                          max_pages, n_slots, n_pages, n_heads, n_kv_heads, dk, dv, window, chunk, keep_first, splits, out_f32, scale, softcap,
+                          max_pages, n_slots, n_pages, n_heads, n_kv_heads, dk, dv, window, chunk, keep_first, splits, max_context, out_f32, scale, softcap,
                           softcap > 0.f ? 2.f * 1.4426950408889634f / softcap : 0.f, q_aligned, status};
 #define GO(T) do { if (dk <= 64 && dv <= 128) return go<T, 1, 1, 8, false>(p, T_tokens, stream); \
                    if (dk == 128 && dv == 128) return go<T, 2, 1, 8, true>(p, T_tokens, stream); \

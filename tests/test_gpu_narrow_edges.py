@@ -103,3 +103,23 @@ def test_a_row_with_a_sink_does_not_depend_on_its_batch(size, dtype):
             for reach in (lens[r], 128, 256, 300):
                 assert torch.equal(run([r], reach, out_dtype=out_dtype)[0], whole[r]), (r, reach)
     assert int(status.item()) == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", [64, 256, 20])                 # of a head: 256 and 128 keys to a split, and the plain kernel
+@pytest.mark.parametrize("reach", [1, 100, 200, 256, 257, 600])
+def test_positions_from_the_context_on_are_reported(reach, size, dtype):
+    rng = np.random.default_rng(22)
+    pages = U.paged(rng, [700, 700], 1, size, size)
+    dev, table = device(pages)
+    q = torch.tensor(rng.normal(size=(2, 2 * size))).to(TYPES[dtype]).cuda()
+    run = lambda rows, pos, status: kv8.decode(q[rows], 2, 1, size, size ** -0.5, 0, i32(rows), i32(pos), table, 64, *dev, reach, status)   # noqa: E731
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    last = run([0], [reach - 1], status)
+    assert int(status.item()) == 0
+    want, bound = U.attention(U.f64(q[:1]).reshape(1, 2, size), pages[:2], pages[2:4], [0], [reach - 1], pages[4], 2, size ** -0.5, wide_weights=dtype == "f32", out_bf16=dtype == "bf16")
+    close(last, want, bound)
+    for beyond in (reach, reach + 1, 699):
+        status.zero_()
+        got = run([0, 1], [reach - 1, beyond], status)
+        assert int(status.item()) == 1 and (got[1] == 0).all() and torch.equal(got[:1], last), beyond
