@@ -129,8 +129,10 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     // work, so the last ones to start are the shortest (a causal tile's work grows with its position)
     const TileInfo tile = tiles[blockIdx.y];
     if (tile.n_rows <= 0) return;             // an unused entry of a tile list of fixed length (captured steps): the whole CTA leaves
-    if (NARROW && (tile.n_rows > BM || tile.slot < 0 || tile.slot >= codes.n_slots || tile.qpos0 < 0 || (tile.qpos0 + tile.n_rows - 1) / BN >= max_pages ||
-                   tile.row_start < 0 || tile.row_start + tile.n_rows > codes.rows)) {       // report, touch nothing
+    // (sums without a sign: a first row or position near 2^31 stays large)
+    if (NARROW && (tile.n_rows > BM || tile.slot < 0 || tile.slot >= codes.n_slots || tile.qpos0 < 0 ||
+                   ((uint32_t)tile.qpos0 + tile.n_rows - 1) / BN >= (uint32_t)max_pages ||
+                   tile.row_start < 0 || (uint32_t)tile.row_start + tile.n_rows > (uint32_t)codes.rows)) {       // report, touch nothing
         if (threadIdx.x == 0 && blockIdx.x == 0) atomicExch(status, 1);
         return;
     }

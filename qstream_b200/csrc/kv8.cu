@@ -354,11 +354,14 @@ kv8_attention_kernel(TO* __restrict__ out, const T* __restrict__ q, const Attend
         const int32_t* t = p.tiles + 4 * (blockIdx.y >> 7);
         const int i = blockIdx.y & 127;
         if (i >= t[1]) return;
-        row = t[0] + i; pos = t[2] + i; slot = t[3];
-        if (t[1] > 128 || t[0] < 0 || t[0] + t[1] > p.T || slot < 0 || slot >= p.n_slots || t[2] < 0 || (t[2] + t[1] - 1) >> 6 >= p.max_pages) {      // the whole tile: report, write nothing
+        slot = t[3];
+        // the whole tile: report, write nothing (sums without a sign: a first row or position near 2^31 stays large)
+        if (t[1] > 128 || t[0] < 0 || (uint32_t)t[0] + t[1] > (uint32_t)p.T || slot < 0 || slot >= p.n_slots || t[2] < 0 ||
+            ((uint32_t)t[2] + t[1] - 1) >> 6 >= (uint32_t)p.max_pages) {
             if (lane == 0) atomicExch(p.status, 1);
             return;
         }
+        row = t[0] + i; pos = t[2] + i;
     } else {
         row = blockIdx.y; slot = p.tok_slot[row]; pos = p.tok_pos[row];
     }

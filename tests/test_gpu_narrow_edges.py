@@ -123,3 +123,18 @@ def test_positions_from_the_context_on_are_reported(reach, size, dtype):
         status.zero_()
         got = run([0, 1], [reach - 1, beyond], status)
         assert int(status.item()) == 1 and (got[1] == 0).all() and torch.equal(got[:1], last), beyond
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_tiles_at_the_end_of_32_bits_are_reported(dtype):
+    """A first row or position whose sum with the number of rows has no place in 32 bits."""
+    rng = np.random.default_rng(23)
+    pages = U.paged(rng, [200], 1, 64, 64)
+    dev, table = device(pages)
+    q = torch.tensor(rng.normal(size=(20, 64))).to(TYPES[dtype]).cuda()
+    top = 2 ** 31 - 1
+    for bad in ((top, 5, 0, 0), (top - 4, 5, 0, 0), (top - 100, 128, 0, 0), (10, 5, top, 0), (10, 5, top - 3, 0), (10, top, 0, 0), (-2 ** 31, 5, 0, 0), (10, 5, -2 ** 31, 0)):
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        out = torch.full((20, 64), 7.0, dtype=TYPES[dtype], device="cuda")
+        kv8.prefill(q, 1, 1, 64, 0.125, 0, i32([bad]), table, 64, *dev, status, out=out)
+        assert int(status.item()) == 1 and (out == 7).all(), bad
