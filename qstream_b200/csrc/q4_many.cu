@@ -351,7 +351,9 @@ q4_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
                 }
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                y[k] = y[k] * row_unit[k] * unit + bias[k];
+                // one power large, the other small: together first, or what comes between has no place in 32 bits
+                y[k] = (row_unit[k] > 1.f) != (unit > 1.f) ? y[k] * (row_unit[k] * unit) : y[k] * row_unit[k] * unit;
+                y[k] += bias[k];
                 if (p.act != QS_ACT_NONE) y[k] = activated(y[k], p.act);
                 y[k] += add[k];
             }

@@ -138,3 +138,16 @@ def test_tiles_at_the_end_of_32_bits_are_reported(dtype):
         out = torch.full((20, 64), 7.0, dtype=TYPES[dtype], device="cuda")
         kv8.prefill(q, 1, 1, 64, 0.125, 0, i32([bad]), table, 64, *dev, status, out=out)
         assert int(status.item()) == 1 and (out == 7).all(), bad
+
+
+@pytest.mark.parametrize("m", [40, 130])
+@pytest.mark.parametrize("x_size,w_size", [(2.0 ** -105, 2.0 ** 122), (2.0 ** 122, 2.0 ** -122), (2.0 ** -100, 2.0 ** 80), (2.0 ** 60, 2.0 ** 50), (2.0 ** -60, 2.0 ** -50)])
+def test_powers_of_two_of_rows_and_matrix_far_apart(x_size, w_size, m):
+    """Large scales beside small rows and the other way round, where the results lie within 32 bits."""
+    n, k = 5000, 4096
+    w = q4.quantize(normal(1, n, k) * w_size, 64)
+    x = (normal(2, m, k) * x_size).bfloat16()
+    assert torch.isfinite(w.scales.float()).all() and (w.scales != 0).any()
+    want, bound = U.linear(U.f64(x), U.dense(w), out_bf16=True)
+    got = U.f64(q4.linear(x, w, out_dtype=torch.float32))
+    assert (np.abs(got - want) <= bound).all(), float(np.nanmax(np.abs(got - want) / bound))
