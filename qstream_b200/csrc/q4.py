@@ -19,6 +19,7 @@ from . import gemm_tc, ops
 GROUPS = (32, 64, 128)
 TYPES = (torch.float32, torch.bfloat16)
 MAX_COLUMNS = 32768
+MAX_ROWS = 65408                    # of a call to the library: what the kernels' grids hold, in whole tiles of 128
 
 _quantize = _linear = _scratch = _kernels = None
 
@@ -143,6 +144,11 @@ def linear(x, weight: Weight4, bias=None, activation=None, residuals=(), out_dty
     else:
         out, r0, r1, ldr = torch.empty((M, N), dtype=want, device=x.device), None, None, N
     if M == 0:
+        return out
+    if M > MAX_ROWS:
+        for a in range(0, M, MAX_ROWS):
+            part = [None if t is None else t[a:a + MAX_ROWS] for t in (x, out, r0, r1)]
+            linear(part[0], weight, bias, activation, part[2:], out=part[1], settled=settled)
         return out
     codes, scales = weight._codes, weight._scales
     stream = launch_stream(codes.get_device(), x, bias, out, r0, r1)

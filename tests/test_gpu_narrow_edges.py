@@ -151,3 +151,17 @@ def test_powers_of_two_of_rows_and_matrix_far_apart(x_size, w_size, m):
     want, bound = U.linear(U.f64(x), U.dense(w), out_bf16=True)
     got = U.f64(q4.linear(x, w, out_dtype=torch.float32))
     assert (np.abs(got - want) <= bound).all(), float(np.nanmax(np.abs(got - want) / bound))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,k", [(16, 64), (24, 100), (300, 64)])
+def test_more_rows_than_a_grid_holds(n, k, dtype):
+    t, m = TYPES[dtype], 140000
+    w = q4.quantize(normal(1, n, k, std=0.1), 32)
+    x, bias, r0 = normal(2, m, k, dtype=t), normal(3, n), normal(4, m, n, dtype=t)
+    want, bound = U.linear(U.f64(x), U.dense(w), U.f64(bias), None, [U.f64(r0)], out_bf16=t == torch.bfloat16)
+    got = q4.linear(x, w, bias, residuals=(r0,))
+    assert (np.abs(U.f64(got) - want) <= bound).all()
+    out = torch.full((m, n + 3), 7.0, dtype=t, device="cuda")
+    assert q4.linear(x, w, bias, residuals=(None, r0), out=out[:, 1:1 + n]).data_ptr() == out[:, 1:].data_ptr()
+    assert torch.equal(out[:, 1:1 + n], got) and (out[:, 0] == 7).all() and (out[:, 1 + n:] == 7).all()
