@@ -101,11 +101,13 @@ def launch_stream(device: int, *tensors) -> int:
 
 def quantize(weight: torch.Tensor, group: int = 64) -> Weight4:
     """Round a float32 or bfloat16 matrix (any row stride) to 4 bits.  Of each row's group, the element m of the largest magnitude sets the
-    scale s = bfloat16(-m / 8); a weight w becomes the nearest (ties to even) of the numbers -8 s .. 7 s."""
+    scale s = bfloat16(-m / 8); a weight w becomes the nearest (ties to even) of the numbers -8 s .. 7 s.  Up to 32,768 columns, as `linear` takes them."""
     if weight.dim() != 2 or weight.stride(1) != 1 or weight.dtype not in TYPES or 0 in weight.shape:
         _refuse(f"4-bit weights: need a float32 or bfloat16 matrix with contiguous rows, got {weight.dtype} {tuple(weight.shape)} strides {weight.stride()}")
     if group not in GROUPS:
         _refuse(f"4-bit weights: groups of {group} columns (groups: {GROUPS})", QsError.QUANT_MISMATCH)
+    if weight.shape[1] > MAX_COLUMNS:
+        _refuse(f"4-bit weights: a matrix of {weight.shape[1]} columns, the products take {MAX_COLUMNS}", QsError.QUANT_MISMATCH)
     stream = launch_stream(weight.get_device())
     _bind()
     N, K = weight.shape

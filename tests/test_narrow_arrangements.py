@@ -43,3 +43,13 @@ def test_what_a_key_takes_does_not_depend_on_how_the_matrices_are_held(tmp_path,
         for bits in (None, 4):
             mixer = qs.load_model(folder, dtype=dtype, device="cpu", allow_mmap=False, weight_bits=bits).blocks[0].mixer
             assert mixer.cache_bytes_per_key == size * mixer.spec.n_kv_heads * (mixer.spec.head_dim + mixer.spec.value_dim)
+
+
+def test_a_matrix_that_no_product_takes_is_not_made():
+    """Wider matrices are refused when they are rounded, so when a model is loaded, and not at its first step."""
+    from qstream_b200.parts import Runtime
+    wide = torch.zeros(2, q4.MAX_COLUMNS + 1)
+    for make in (q4.quantize, Runtime(dtype=torch.float32, device=torch.device("cpu"), weight_group=64).matrix):
+        with pytest.raises(QStreamError, match="32769 columns") as e:
+            make(wide)
+        assert e.value.code == QsError.QUANT_MISMATCH
