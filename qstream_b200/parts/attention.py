@@ -92,7 +92,7 @@ class Attention(Mixer):
             mats.append(torch.zeros((pad, spec.width), dtype=mats[0].dtype, device=mats[0].device))
         if len({m.dtype for m in mats}) != 1:
             raise QStreamError(QsError.INVALID_MODEL, "q/k/v projections are stored in different types")
-        self.w_qkv = runtime.matrix(torch.cat(mats, dim=0).contiguous() if len(mats) > 1 else mats[0])
+        self.w_qkv = runtime.matrix(torch.cat(mats, dim=0).contiguous() if len(mats) > 1 else mats[0], pad)
         self.b_qkv = None
         if spec.qkv_bias:
             biases = [tensors[n + "_bias"].float() for n in names]

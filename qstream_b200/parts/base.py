@@ -68,13 +68,13 @@ class Runtime:
     weight_group: int = 0               # g > 0: the matrices of attention and dense feed-forwards in 4 bits, a scale for each g columns
     narrowed: list = field(default_factory=list, compare=False)        # (bytes before, bytes after) of every matrix that `matrix` rounded
 
-    def matrix(self, weight: torch.Tensor):
-        """A part's matrix as its products take it: as it is, or rounded to 4 bits."""
+    def matrix(self, weight: torch.Tensor, filled_rows: int = 0):
+        """A part's matrix as its products take it: as it is, or rounded to 4 bits.  The last `filled_rows` rows are none of the model's."""
         if not self.weight_group:
             return weight
         from ..csrc import q4
         narrow = q4.quantize(weight, self.weight_group)
-        self.narrowed.append((weight.numel() * weight.element_size(), narrow.nbytes))
+        self.narrowed.append((weight[:weight.shape[0] - filled_rows].numel() * weight.element_size(), narrow.nbytes))
         return narrow
 
 

@@ -53,3 +53,26 @@ def test_a_matrix_that_no_product_takes_is_not_made():
         with pytest.raises(QStreamError, match="32769 columns") as e:
             make(wide)
         assert e.value.code == QsError.QUANT_MISMATCH
+
+
+@pytest.mark.parametrize("name,which", [m for m in MODELS if m[0] in ("lutelorn", "fotanex", "vofinex") and m not in WIDE_ONLY])
+def test_the_bytes_of_a_narrow_model(tmp_path, monkeypatch, name, which):
+    """What the wide model holds, less its matrices, and the narrow ones; rows that fill up a product are none of the wide model's."""
+    from qstream_b200.parts import Part
+    monkeypatch.setattr(q4, "quantize", rounded)
+    folder, _ = importlib.import_module(name + "_util").make_folder(tmp_path, which, "float32")
+    wide, narrow = (qs.load_model(folder, dtype="float32", device="cpu", allow_mmap=False, weight_bits=bits) for bits in (None, 4))
+    stored = held = 0
+
+    def look(part):
+        nonlocal stored, held
+        for key, value in vars(part).items():
+            if isinstance(value, q4.Weight4):
+                rows = part.gate_at + part.gate_rows if key == "w_qkv" else value.out_features
+                stored, held = stored + 4 * rows * value.in_features, held + value.nbytes
+            elif isinstance(value, Part):
+                look(value)
+
+    for block in narrow.blocks:
+        look(block)
+    assert narrow.weight_bytes == wide.weight_bytes - stored + held
