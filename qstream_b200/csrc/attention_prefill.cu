@@ -28,6 +28,7 @@
 // Sizes: head size a multiple of 16 up to 256 (tiles are padded to 64 columns with TMA's zero fill);
 // any number of heads and groups; pages of 64 tokens.
 #include "common.cuh"
+#include "per_device.h"
 #include "sm100.cuh"
 
 #include <mutex>
@@ -550,14 +551,15 @@ int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, 
            const TileInfo* tiles, int n_tiles, const int32_t* page_table, int max_pages, int n_heads, int n_kv_heads,
            int dh, float scale_log2, int window, int32_t* status, int dv, float cap_log2, float cap_k2, const void* gate,
            long long ldg, const MaskOpts& mask, const Codes& codes, cudaStream_t stream) {
-    static bool configured = false;
-    if (!configured) {
-        cudaError_t e = cudaFuncSetAttribute(attention_prefill_kernel<NKC, NARROW>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             smem_bytes<NKC>());
-        if (e != cudaSuccess) return qs_fail(QS_ERR_INTERNAL, "attention_prefill: shared memory of %d bytes refused: %s",
-                                             smem_bytes<NKC>(), cudaGetErrorString(e));
-        configured = true;
-    }
+    static PerDevice limit;
+    int device = 0;
+    cudaGetDevice(&device);
+    cudaError_t e = cudaSuccess;
+    if (!limit.get(device, [&] {
+            e = cudaFuncSetAttribute(attention_prefill_kernel<NKC, NARROW>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<NKC>());
+            return e == cudaSuccess ? 1 : 0;
+        }))
+        return qs_fail(QS_ERR_INTERNAL, "attention_prefill: shared memory of %d bytes refused: %s", smem_bytes<NKC>(), cudaGetErrorString(e));
     attention_prefill_kernel<NKC, NARROW><<<dim3(n_heads, n_tiles), THREADS + NARROW * DECODERS * 32, smem_bytes<NKC>(), stream>>>(
         mq, mk, mv, (__nv_bfloat16*)out, (size_t)ldo, tiles, page_table, max_pages, n_heads, n_kv_heads, dh,
         scale_log2, window, status, dv, cap_log2, cap_k2, (const __nv_bfloat16*)gate, (size_t)ldg, mask, codes);

@@ -40,3 +40,8 @@ def test_each_device_is_asked_for_itself(tmp_path):
 def test_the_float32_product_asks_per_device():
     source = (CSRC / "linear_split.cu").read_text()
     assert "PerDevice" in source and "static int state" not in source
+
+
+def test_the_attention_of_prompts_asks_per_device():
+    source = (CSRC / "attention_prefill.cu").read_text()
+    assert "PerDevice" in source and "static bool" not in source
