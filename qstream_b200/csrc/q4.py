@@ -122,7 +122,11 @@ def linear(x, weight: Weight4, bias=None, activation=None, residuals=(), out_dty
     """act(x W^T + bias) + residuals for rows x [M, in_features] of float32 or bfloat16, accumulated in 32 bits.  Arguments and
     result as for `parts.linear.linear`: up to two residuals of x's type; `out_dtype` float32 for a 32-bit result; `out`: a view to
     write into (contiguous rows, any row stride).  `settled`: the weight was complete before the previous kernel of the stream began
-    (a model's is); the kernel then fetches it while that kernel still runs."""
+    (a model's is); the kernel then fetches it while that kernel still runs.
+
+    Products are exact and summed in 32 bits, but for one limit: more than 16 bfloat16 rows in a large product are taken as 16-bit floats over a power of
+    two for each row, and so are the scales of a row of the matrix.  A number is off by 2^-25 of its row's largest at most (bfloat16 numbers down to 2^-17
+    of it not at all), a weight by eight times 2^-25 of the largest scale in its row."""
     M, K, ldx = ops._rows(x)
     N, dtype = weight.out_features, x.dtype
     wide = dtype is torch.float32

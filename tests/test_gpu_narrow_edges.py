@@ -5,6 +5,7 @@ import torch
 
 import narrow_util as U
 from qstream_b200.csrc import kv8, q4
+from test_gpu_kv8 import MASKS
 
 pytestmark = pytest.mark.gpu
 TYPES = {"bf16": torch.bfloat16, "f32": torch.float32}
@@ -27,6 +28,16 @@ def close(got, want, bound, what=None):
     assert (err <= bound).all(), (what, float(np.nanmax(err / np.maximum(bound, 1e-300))))
 
 
+def reference(q, pages, slot, pos, per, scale, dtype, bf16_weights, **opts):
+    """`narrow_util.attention`.  Prompts of bfloat16 rows on the tensor cores round each weight to bfloat16, by 2^-8 of it at most; their sum is taken of
+    the weights before that.  So a result moves by 2^-8 of the sum of p |v|, which is the attention over the values' sizes."""
+    want, bound = U.attention(q, pages[:2], pages[2:4], slot, pos, pages[4], per, scale, wide_weights=dtype == "f32" or bf16_weights, out_bf16=dtype == "bf16", **opts)
+    if bf16_weights:
+        sizes, more = U.attention(q, (pages[0], np.abs(pages[1])), pages[2:4], slot, pos, pages[4], per, scale, **opts)
+        bound = bound + (1 + 2.0 ** -8) * 2.0 ** -8 * (sizes + more)
+    return want, bound
+
+
 class Scaled:
     """Keys of 2^e against queries of 2^-e, beside values of as much (as far as 150 of them have a sum): what attention makes of pages is what they read back as."""
 
@@ -39,18 +50,16 @@ class Scaled:
         self.q = (torch.tensor(rng.normal(size=(21, 4 * size))) * 2.0 ** (-e - 6)).to(TYPES[dtype]).cuda()
         self.status = torch.zeros(1, dtype=torch.int32, device="cuda")
 
-    def run(self, call, rounding=0.0, **rows):
+    def run(self, call, bf16_weights=False, **rows):
         dev, table = device(self.pages)
         got = call(self.q, 4, 2, self.size, self.size ** -0.5, 0, **rows, page_table=table, page_tokens=64, k_cache=dev[0], v_cache=dev[1], k_scale=dev[2], v_scale=dev[3],
                    status=self.status)
-        want, bound = U.attention(U.f64(self.q).reshape(21, 4, self.size), self.pages[:2], self.pages[2:4], self.slot, self.pos, self.pages[4], 2, self.size ** -0.5,
-                                  wide_weights=self.dtype == "f32", out_bf16=self.dtype == "bf16")
-        close(got, want, bound + rounding * 127 * 2.0 ** self.e_v)
+        want, bound = reference(U.f64(self.q).reshape(21, 4, self.size), self.pages, self.slot, self.pos, 2, self.size ** -0.5, self.dtype, bf16_weights)
+        close(got, want, bound)
         assert int(self.status.item()) == 0
 
     def prompts(self):
-        # weights rounded to bfloat16 on the tensor cores' path: each of them by half a step, 2^-9 of it, at most
-        self.run(kv8.prefill, 2.0 ** -9 if self.dtype == "bf16" and self.size % 16 == 0 else 0.0, tiles=i32([(0, 20, 130, 0), (20, 1, 63, 1)]))
+        self.run(kv8.prefill, self.dtype == "bf16" and self.size % 16 == 0, tiles=i32([(0, 20, 130, 0), (20, 1, 63, 1)]))
 
     def single_tokens(self):
         self.run(kv8.decode, tok_slot=i32(self.slot), tok_pos=i32(self.pos), max_context=150)
@@ -165,3 +174,50 @@ def test_more_rows_than_a_grid_holds(n, k, dtype):
     out = torch.full((m, n + 3), 7.0, dtype=t, device="cuda")
     assert q4.linear(x, w, bias, residuals=(None, r0), out=out[:, 1:1 + n]).data_ptr() == out[:, 1:].data_ptr()
     assert torch.equal(out[:, 1:1 + n], got) and (out[:, 0] == 7).all() and (out[:, 1 + n:] == 7).all()
+
+
+@pytest.mark.parametrize("H,G,dk,dv", [(1, 1, 64, 64), (4, 2, 128, 128), (3, 1, 64, 32), (2, 1, 256, 256), (2, 2, 80, 48), (4, 1, 144, 192)])
+def test_prompts_are_off_by_the_rounding_of_their_weights_and_no_more(H, G, dk, dv):
+    new, held = [1, 130, 64, 300, 7], [0, 0, 63, 100, 250]
+    lens = [a + b for a, b in zip(new, held)]
+    rng = np.random.default_rng(H * dk + dv + 1)
+    pages = U.paged(rng, lens, G, dk, dv)
+    dev, table = device(pages)
+    slot, pos, tiles, row = [], [], [], 0
+    for i, (n, h) in enumerate(zip(new, held)):
+        tiles += [(row + a, min(128, n - a), h + a, i) for a in range(0, n, 128)]
+        slot, pos, row = slot + [i] * n, pos + list(range(h, h + n)), row + n
+    q = torch.tensor(rng.normal(size=(row, H * dk))).bfloat16().cuda()
+    sink = torch.tensor(rng.normal(size=H) + 1, dtype=torch.float32).cuda()
+    for opts in MASKS:
+        for s in (None, sink):
+            status = torch.zeros(1, dtype=torch.int32, device="cuda")
+            args = dict(opts)
+            got = kv8.prefill(q, H, G, dk, dk ** -0.5, args.pop("window", 0), i32(tiles), table, 64, *dev, status, v_head_dim=dv, sink=s, **args)
+            want, bound = reference(U.f64(q).reshape(row, H, dk), pages, slot, pos, H // G, dk ** -0.5, "bf16", True, sink=None if s is None else U.f64(s), **opts)
+            close(got, want, bound, (opts, s is not None))
+            assert np.median(bound) < 0.25 * np.median(np.abs(want))        # a kernel that returned something else would show
+            assert int(status.item()) == 0
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("m", [33, 200])
+def test_products_of_many_rows_with_outliers(m, group):
+    """Rows whose largest number meets weights of zero, beside numbers down to 2^-40 of it, and groups of very different scales in one row of the
+    matrix.  As 16-bit floats a number is off by 2^-25 of its row's largest at most, and a weight by eight times 2^-25 of its row's largest scale."""
+    n, k = 1200, 16384
+    wf = normal(1, n, k) * torch.logspace(-9, 0, k // 128, base=10.0, device="cuda").repeat_interleave(128)
+    wf[:, 7] = 0
+    w = q4.quantize(wf, group)
+    dense = U.dense(w)
+    assert (dense[:, 7] == 0).all()
+    x = (normal(2, m, k) * 2.0 ** -torch.randint(0, 40, (m, k), generator=torch.Generator().manual_seed(3)).cuda()).bfloat16()
+    x[:, 7] = 2.0 ** 20 * (1 + torch.rand(m, generator=torch.Generator().manual_seed(4))).cuda()
+    want, bound = U.linear(U.f64(x), dense, out_bf16=False)
+    size, scale = np.abs(U.f64(x)), np.abs(U.unpack(w)[1][:n]).max(axis=1)
+    off = 2.0 ** -25 * (size.max(axis=1)[:, None] * np.abs(dense).sum(axis=1)[None] + 8 * (1 + 2.0 ** -10) * size.sum(axis=1)[:, None] * scale[None])
+    got = U.f64(q4.linear(x, w, out_dtype=torch.float32))
+    assert (np.abs(got - want) <= bound + off).all(), float((np.abs(got - want) / (bound + off)).max())
+    # up to 16 rows the numbers are taken as they are
+    few = U.f64(q4.linear(x[:16], w, out_dtype=torch.float32))
+    assert (np.abs(few - want[:16]) <= bound[:16]).all()
