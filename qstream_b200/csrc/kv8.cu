@@ -124,8 +124,8 @@ __device__ __forceinline__ float max_size(float a, float b) {
 }
 
 // n rows of one page and head, from row `a` of the page on: the scale that holds them and what is there already, then the codes.
-// VEC: value(i, d, x) gives elements d .. d + 15 of new row i, else element d.  The rows are read twice, the second time from the caches: they are too
-// many for the registers of a block, and the rotation is cheap.
+// VEC: value(i, d, x) gives elements d .. d + 15 of new row i, else element d.  The rows are read and rotated twice, the second time from the
+// caches (64 bfloat16 rows of 256 numbers would fit a block's registers, 32 of each thread's; that form is not built).
 // Bound by the instructions as much as by memory: some fourteen for an element, seven of them its way through 32 bits and into the maximum, one and three
 // quarters its rounding and packing.
 template <bool VEC, typename F>

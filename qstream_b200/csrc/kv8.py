@@ -77,8 +77,9 @@ def rope_store(q, k, v, n_heads, n_kv_heads, head_dim, rotary_dim, cos_sin, tok_
                k_scale, v_scale, status, v_head_dim=None, v_first=None, v_mix=0.0, half_layout=False, q_out=None) -> None:
     """Rotate q (in place, or into `q_out`) and k, and write k and v into the 8-bit cache; arguments as for `ops.rope_store`, with the
     scales beside the caches.  Keys and values are rounded once, from 32 bits.  Rows with a slot below 0 are padding: their queries stay
-    as they are, nothing is written for them.  A sequence's new tokens are consecutive rows with ascending positions; a page that
-    a second run of rows names in the same call gets the first run only, and status 5."""
+    as they are, nothing is written for them.  A sequence's new tokens are consecutive rows with ascending positions; a second run of rows of a
+    sequence for one page in the same call is not written, and status 5.  Two sequences may share pages that a call does not write; a page that both
+    write to in one call holds neither's tokens reliably."""
     what = "kv8.rope_store"
     dv = int(v_head_dim or head_dim)
     n_pages = _check_cache(what, k_cache, v_cache, k_scale, v_scale, n_kv_heads, head_dim, dv, page_tokens)
@@ -174,7 +175,10 @@ def decode(q, n_heads, n_kv_heads, head_dim, scale, window, tok_slot, tok_pos, p
     """Each row of q [T, n_heads * head_dim] against the 8-bit cache of its sequence, up to the row's own position: softmax(scale q.K) V.
     Masks, cap and sinks as for `attention_bf16.decode`: a window of the last keys, beside it the first `keep_first`; chunks of positions;
     scores c tanh(s / c); exp(sink) in each head's sum.  Positions lie below `max_context`; a row beyond it, or beyond the page table,
-    gives zeros and status 1, a page its sequence does not hold status 3.  Rows with a slot below 0 give zeros."""
+    gives zeros and status 1, a page its sequence does not hold status 3.  Rows with a slot below 0 give zeros.
+
+    Head sizes that are multiples of 16 up to 256 go to the tensor cores, a query as 16-bit floats over a power of two (numbers below 2^-14 of its largest are off
+    by 2^-25 of it; float32 queries are two such floats, 22 bits), bfloat16 rows' weights as 16-bit floats; sums have 32 bits."""
     what = "kv8.decode"
     dv = int(v_head_dim or head_dim)
     T, n_pages, out = _check_attention(what, q, n_heads, n_kv_heads, head_dim, window, page_table, page_tokens, k_cache, v_cache, k_scale, v_scale, status, out, dv,
@@ -212,7 +216,10 @@ def decode(q, n_heads, n_kv_heads, head_dim, scale, window, tok_slot, tok_pos, p
 def prefill(q, n_heads, n_kv_heads, head_dim, scale, window, tiles, page_table, page_tokens, k_cache, v_cache, k_scale, v_scale, status,
             padded=False, out=None, v_head_dim=None, softcap=0.0, chunk=0, keep_first=0, sink=None, out_dtype=None) -> torch.Tensor:
     """Many rows per sequence against the 8-bit cache.  `tiles` (int32 [n, 4]: first row, number of rows up to 128, position of the first row,
-    slot) as from `attention_bf16.prefill_tiles`; rows that no tile covers are left as they are, or zeros with `padded`.  The rest as for `decode`."""
+    slot) as from `attention_bf16.prefill_tiles`; rows that no tile covers are left as they are, or zeros with `padded`.  The rest as for `decode`.
+
+    bfloat16 rows go to the tensor cores (head sizes that are multiples of 16 up to 256), their softmax weights rounded to bfloat16.  float32 rows and other head sizes take
+    the plain kernel, a warp for a row and head: three prompts, 2,047 rows of 16 heads of 128: 5.9 ms, where bfloat16 rows take 39 us."""
     what = "kv8.prefill"
     dv = int(v_head_dim or head_dim)
     T, n_pages, out = _check_attention(what, q, n_heads, n_kv_heads, head_dim, window, page_table, page_tokens, k_cache, v_cache, k_scale, v_scale, status, out, dv,

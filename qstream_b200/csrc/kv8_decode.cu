@@ -5,7 +5,7 @@
 // Floor: the bytes of the pages.  A warp takes 32 keys and up to HEADS query heads that share their key head: a bulk
 // copy brings the keys into shared memory, asynchronous copies the values, their rows apart (all of a block are on their way at once, from
 // the first instructions on); 16-bit products on mma.m16n8k16 take them from there.  Bound by a block's life: its metadata's and pages' way from
-// memory, one behind the other, then instructions, which fill two fifths of the slots.  (Blocks that stay on their SM and look for their next
+// memory, one behind the other, then instructions, which fill half of the slots (heads of 128; two fifths, heads of 256).  (Blocks that stay on their SM and look for their next
 // page's number beside the products: 31 rows of 2,048 29 us instead of 25 without the merge; they wait and compute all at the same time.)
 //
 //   scores   left operand: 16 keys, right: the heads.  A lane's 16 bytes of a key's row are its part of four steps; which dims meet in

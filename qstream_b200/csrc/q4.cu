@@ -18,9 +18,10 @@ long long q4_many_scratch(int M, int N, int chunks);
 
 namespace {
 
-// Which bfloat16 products go to the 5th-generation tensor cores: those of more than 16 rows that are large enough for what they take beside (some 12 us for the
-// powers of two, the way of the first chunk and of the results).  Microseconds, 16 rows at a time here | there: 32 rows, 2,048 x 2,048: 7 | 17, 4,096 x 4,096:
-// 13 | 16, 16,384 x 4,096: 42 | 36, 4,096 x 16,384: 53 | 39; 64 rows: 12 | 19, 27 | 17, 84 | 37, 101 | 41.
+// Which bfloat16 products go to the 5th-generation tensor cores: those of more than 16 rows that are large enough for what they take beside (some 11 us for the
+// powers of two, the way of the first chunk and of the results).  Microseconds, 16 rows at a time here | there, matrices of 2,048 x 2,048, 4,096 x 4,096,
+// 8,192 x 2,048, 16,384 x 4,096 and 4,096 x 16,384: 32 rows 7 | 16, 14 | 14, 13 | 13, 42 | 28, 52 | 31; 64 rows 13 | 17, 27 | 15, 24 | 15, 82 | 30, 102 | 33;
+// 128 rows of the first 23 | 21.
 bool many_rows(int M, int N, int K, int dtype) { return dtype == QS_BF16 && M > 16 && (double)M * N * K >= 6e8; }
 
 // The column within eight of a word's i-th code.
